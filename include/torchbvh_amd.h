@@ -537,6 +537,79 @@ int tbvh_interpolate_backward(const float* grad, const int64_t* indices, const f
                               void* stream);
 
 
+/* ---- attention over blocks of a curve order --------------------------------------
+ * No counterpart in the reference.  Rows (points, features) are packed cloud
+ * after cloud in curve order and cut into blocks that never straddle two clouds:
+ * `starts` (blocks + 1, int64, device) holds each block's first row, `clouds`
+ * (clouds + 1, int64, device) each cloud's first block.  A block holds at most
+ * its layout's block size; rows past it, past the next block's start or past the
+ * tensor are not read, whatever the arrays hold. */
+
+/* Nearest key blocks of every block of queries: out (groups, count) int32, the
+ * `count` (1 to 64) blocks of the group's cloud with the least squared distance
+ * from the centre of the queries' box to the block's box, ascending by (distance,
+ * block number), -1 where there are fewer.  queries (q_rows, D), boxes (blocks,
+ * 2D: lo, hi) fp32, D 2 or 3; both layouts have the same clouds. */
+int tbvh_select_blocks_workspace_size(int64_t blocks, int D, size_t* bytes);
+int tbvh_select_blocks(const float* queries, int64_t q_rows, const int64_t* q_starts, const int64_t* q_clouds,
+                       int64_t groups, int64_t q_block, const float* boxes, const int64_t* k_clouds, int64_t blocks,
+                       int64_t clouds, int D, int count, int32_t* out, void* workspace, size_t workspace_bytes,
+                       void* stream);
+
+/* Attention of every query row over the rows of the key blocks chosen for its
+ * block, softmax(scale q.k + bias) v, in bf16 (bf16 = 1) or fp32; a row that is
+ * given no keys is zero.  Query head h reads key head h / (heads / kv_heads).
+ * Strides are in elements, multiples of 16 bytes, and channels are contiguous; D
+ * is a multiple of 8 up to 128.  out, and the backward's gradients, are
+ * contiguous.  `selected` entries outside [0, blocks) choose nothing.
+ *
+ * Bias (table not null): sum over axes a of table[a, map[clamp(q_cells[i, a] -
+ * k_cells[j, a], -reach, reach) + reach], h]; table (axes, buckets, heads) of q's
+ * type, map (2 reach + 1) and cells (rows, axes) int32, axes 1 to 3, axes * buckets
+ * at most 256, heads / kv_heads * axes * (2 reach + 1) at most 4096.
+ *
+ * lse (q_rows, heads), wanted for the backward, may be null. */
+typedef struct tbvh_attend_args {
+    const void *q, *k, *v;
+    int64_t q_row_stride, q_head_stride, k_row_stride, k_head_stride, v_row_stride, v_head_stride;
+    int64_t q_rows, k_rows;
+    const int32_t* selected;
+    const int64_t *q_starts, *k_starts;
+    int64_t groups, blocks;
+    int32_t count, q_block, k_block, heads, kv_heads, D, bf16;
+    float scale;
+    const void* table;
+    const int32_t *map, *q_cells, *k_cells;
+    int32_t axes, buckets, reach;
+    void* out;
+    float* lse;
+} tbvh_attend_args;
+int tbvh_attend(const tbvh_attend_args* args, void* stream);
+
+/* Gradients of tbvh_attend in q, k, v and, with a bias, its table, from `grad` of
+ * `out`; args as in the forward call, with its out and lse. */
+int tbvh_attend_backward_workspace_size(const tbvh_attend_args* args, size_t* bytes);
+int tbvh_attend_backward(const tbvh_attend_args* args, const void* grad, void* dq, void* dk, void* dv, void* dtable,
+                         void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- group norm with an activation ------------------------------------------------
+ * No counterpart in the reference.  x (rows, channels), channels last, bf16 or
+ * fp32; statistics over each cloud's rows (offsets (clouds + 1) int64 on the
+ * device, or null for clouds of equal size) and each of `groups` groups of
+ * channels; y = act(weight xhat + bias), activation 0 none, 1 relu, 2 silu, 3 gelu
+ * (by erf).  weight and bias (channels), of x's type or fp32 (wide_weights = 1),
+ * may be null.  mean, rstd (clouds, groups) fp32 are the forward's outputs and the
+ * backward's inputs; dx, dweight and dbias may be null where not wanted. */
+int tbvh_group_norm_workspace_size(int64_t rows, int64_t clouds, int64_t channels, int64_t groups, size_t* bytes);
+int tbvh_group_norm(const void* x, const int64_t* offsets, int64_t rows, int64_t clouds, int64_t channels,
+                    int64_t groups, const void* weight, const void* bias, int wide_weights, int bf16, float eps,
+                    int activation, void* y, float* mean, float* rstd, void* workspace, size_t workspace_bytes,
+                    void* stream);
+int tbvh_group_norm_backward(const void* x, const void* grad, const int64_t* offsets, int64_t rows, int64_t clouds,
+                             int64_t channels, int64_t groups, const void* weight, const void* bias, int wide_weights,
+                             int bf16, float eps, int activation, const float* mean, const float* rstd, void* dx,
+                             void* dweight, void* dbias, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,118 @@
+"""Block layouts, buckets and the refusals of the block operators and the group
+norm that fire before any GPU work; the 64-bit restatement that the GPU tests
+compare with, against differences."""
+
+import pytest
+import torch
+
+import blocks_reference as ref
+import torchbvh_amd as tb
+
+
+@pytest.mark.parametrize("block", [1, 2, 63, 64, 128])
+@pytest.mark.parametrize("source", [(1, 1), (1, 64), (3, 65), (2, 1000), (4, 0)])
+def test_layout_of_equal_clouds(source, block):
+    layout = tb.block_layout(source, block, device="cpu")
+    offsets, starts, clouds = ref.layout_lists([source[1]] * source[0], block)
+    assert (layout.offsets.tolist(), layout.starts.tolist(), layout.clouds.tolist()) == (offsets, starts, clouds)
+    assert layout.block_size == block
+
+
+@pytest.mark.parametrize("args,match", [
+    (((1, 4), 0), "block_size must be 1 to 128"), (((1, 4), 129), "block_size must be 1 to 128"),
+    (((0, 4),), "need B >= 1"), (("points",), "source must be a handle"),
+    ((torch.zeros(3),), "offsets must be int64"), ((torch.zeros(3, dtype=torch.int64),), "offsets must be a CUDA tensor"),
+])
+def test_layout_refusals(args, match):
+    with pytest.raises(ValueError, match=match):
+        tb.block_layout(*args, device="cpu")
+
+
+@pytest.mark.parametrize("sizes,far", [(2, 1), (2, 40), (8, 5), (16, 24), (16, 128), (31, 1000)])
+def test_buckets(sizes, far):
+    b = tb.relative_buckets(sizes, far, device="cpu")
+    assert b.dtype == torch.int32 and b.numel() == 2 * far + 1 and b[far] == 0
+    up, down = b[far + 1 :], b[:far].flip(0)
+    near = sizes // 2
+    assert up[: min(near, far + 1) - 1].tolist() == list(range(1, min(near, far + 1)))
+    assert (up.diff() >= 0).all() and 0 < up.min() and up.max() <= sizes - 1
+    assert torch.equal(down, up + sizes - 1)  # negative distances mirror positive ones
+    if far > 4 * sizes:
+        assert up[-1] == sizes - 1
+
+
+def rows(n=6, heads=2, d=8):
+    return torch.zeros(n, heads, d)
+
+
+def test_attention_refusals():
+    layout = tb.block_layout((1, 6), 4, device="cpu")
+    chosen = torch.zeros((2, 1), dtype=torch.int32)
+    for q, match in ((torch.zeros(6, 8), "q must have shape"), (rows(), "q must be a CUDA tensor")):
+        with pytest.raises(ValueError, match=match):
+            tb.block_attention(q, rows(), rows(), chosen, layout, layout)
+
+
+def test_norm_and_selection_refusals():
+    x = torch.zeros(2, 3, 8)
+    layout = tb.block_layout((1, 6), 4, device="cpu")
+    for args, match in (((torch.zeros(8), 2), "x must have shape"), ((x, 2, None, None, layout), "x must have shape"),
+                        ((x, 2), "x must be a CUDA tensor")):
+        with pytest.raises(ValueError, match=match):
+            tb.group_norm_act(*args)
+    with pytest.raises(ValueError, match="queries must have shape"):
+        tb.select_blocks(torch.zeros(3), torch.zeros(1, 6), 1, layout, layout)
+    with pytest.raises(ValueError, match="D must be 2 or 3"):
+        tb.select_blocks(torch.zeros(3, 4), torch.zeros(1, 8), 1, layout, layout)
+    with pytest.raises(ValueError, match="queries must be a CUDA tensor"):
+        tb.select_blocks(torch.zeros(3, 2), torch.zeros(1, 4), 1, layout, layout)
+    with pytest.raises(ValueError, match="power of two"):
+        tb.block_boxes({}, 48)
+    with pytest.raises(TypeError):
+        tb.block_boxes({}, 64)
+
+
+def _slope(f, x, d, h=1e-5):
+    return ((f(x + h * d) - f(x - h * d)) / (2 * h)).item()
+
+
+def test_reference_attention_gradients_against_differences():
+    g = torch.Generator().manual_seed(0)
+    q, grad = (torch.randn(5, 4, 8, generator=g, dtype=torch.float64) for _ in range(2))
+    k, v = (torch.randn(7, 2, 8, generator=g, dtype=torch.float64) for _ in range(2))
+    table = torch.randn(2, 5, 4, generator=g, dtype=torch.float64)
+    buckets = torch.tensor([3, 4, 0, 1, 2], dtype=torch.int32)
+    cells = [torch.randint(-3, 4, (n, 2), generator=g) for n in (5, 7)]
+    times = torch.randint(0, 3, (5, 7), generator=g).double()
+    times[2] = 0
+    args = {"q": q, "k": k, "v": v, "table": table}
+
+    def loss(**changed):
+        a = {**args, **changed}
+        out = ref.attention(a["q"], a["k"], a["v"], times, 0.3, (a["table"], buckets, *cells))["out"][0]
+        return (out * grad).sum()
+
+    want = ref.attention(q, k, v, times, 0.3, (table, buckets, *cells), grad)
+    assert not want["out"][0][2].any()
+    for name in args:
+        d = torch.randn(args[name].shape, generator=g, dtype=torch.float64)
+        slope = _slope(lambda x: loss(**{name: x}), args[name], d)
+        # Central differences: an error of h^2 and of 2^-52 / h.
+        assert abs((want["d" + name][0] * d).sum().item() - slope) < 1e-7
+
+
+@pytest.mark.parametrize("activation", ["none", "relu", "silu", "gelu"])
+def test_reference_norm_gradients_against_differences(activation):
+    g = torch.Generator().manual_seed(1)
+    x, grad = (torch.randn(9, 6, generator=g, dtype=torch.float64) for _ in range(2))
+    w, b = (torch.randn(6, generator=g, dtype=torch.float64) for _ in range(2))
+    args = {"x": x, "w": w, "b": b}
+
+    def loss(**changed):
+        a = {**args, **changed}
+        return (ref.group_norm(a["x"], [0, 4, 9], 3, a["w"], a["b"], 1e-5, activation)["out"][0] * grad).sum()
+
+    want = ref.group_norm(x, [0, 4, 9], 3, w, b, 1e-5, activation, grad)
+    for name in args:
+        d = torch.randn(args[name].shape, generator=g, dtype=torch.float64)
+        assert abs((want["d" + name][0] * d).sum().item() - _slope(lambda t: loss(**{name: t}), args[name], d)) < 1e-6

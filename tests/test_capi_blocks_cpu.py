@@ -1,0 +1,135 @@
+"""Argument errors of the C entry points for blocks and the group norm, reported
+(status and message) before anything is launched."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+
+from torchbvh_amd import _native
+
+FAKE = ctypes.c_void_p(0x100000)  # never dereferenced: every call below fails validation
+INVALID, SMALL = 1, 2
+
+
+def _err() -> str:
+    return _native.load().tbvh_last_error().decode()
+
+
+def _select(**changed):
+    a = dict(queries=FAKE, q_rows=10, q_starts=FAKE, q_clouds=FAKE, groups=10, q_block=1, boxes=FAKE, k_clouds=FAKE,
+             blocks=5, clouds=1, D=3, count=4, out=FAKE, ws=FAKE, ws_bytes=0, stream=None) | changed
+    return _native.load().tbvh_select_blocks(*a.values())
+
+
+@pytest.mark.parametrize("changed,match", [
+    ({"D": 4}, "D must be 2 or 3"), ({"count": 0}, "count must be 1 to 64"), ({"count": 65}, "count must be 1 to 64"),
+    ({"q_block": 0}, "1 to 128 rows"), ({"groups": (1 << 26) + 1}, "groups <= 2\\^26"), ({"clouds": 0}, "clouds >= 1"),
+    ({"blocks": 1 << 31}, "blocks in int32"), ({"out": None}, "null"), ({"queries": None}, "null"),
+    ({"boxes": None}, "null"), ({"k_clouds": None}, "null"),
+])
+def test_select_argument_errors(changed, match):
+    assert _select(**changed) == INVALID
+    with pytest.raises(AssertionError, match=match):
+        raise AssertionError(_err())
+
+
+def test_select_workspace():
+    assert _select(ws_bytes=0) == SMALL and "workspace holds 0 bytes" in _err()
+    L = _native.load()
+    n = ctypes.c_size_t(0)
+    assert L.tbvh_select_blocks_workspace_size(1 << 20, 3, ctypes.byref(n)) == 0 and n.value >= (1 << 14) * 24
+    assert L.tbvh_select_blocks_workspace_size(1 << 31, 3, ctypes.byref(n)) == INVALID
+    assert L.tbvh_select_blocks_workspace_size(5, 3, None) == INVALID
+    assert _select(groups=0) == 0
+
+
+def _args(**changed):
+    p = FAKE.value
+    a = dict(q=p, k=p, v=p, q_row_stride=64, q_head_stride=32, k_row_stride=64, k_head_stride=32, v_row_stride=64,
+             v_head_stride=32, q_rows=100, k_rows=100, selected=p, q_starts=p, k_starts=p, groups=2, blocks=2, count=1,
+             q_block=64, k_block=64, heads=2, kv_heads=2, D=32, bf16=0, scale=1.0, out=p, lse=p) | changed
+    return _native.AttendArgs(**a)
+
+
+BIAS = dict(table=FAKE.value, map=FAKE.value, q_cells=FAKE.value, k_cells=FAKE.value, axes=3, buckets=9, reach=8)
+
+
+@pytest.mark.parametrize("changed,match", [
+    ({"D": 12}, "D must be a multiple of 8"), ({"D": 136}, "up to 128"), ({"D": 0}, "multiple of 8"),
+    ({"heads": 3}, "multiple of kv_heads"), ({"kv_heads": 0}, "multiple of kv_heads"), ({"q_block": 129}, "1 to 128 rows"),
+    ({"k_block": 0}, "1 to 128 rows"), ({"q_rows": -1}, ">= 0"), ({"count": -1}, ">= 0"), ({"blocks": 1 << 31}, "int32"),
+    ({"groups": 1 << 25, "count": 64}, "groups \\* count"), ({"groups": 1 << 26, "heads": 8, "kv_heads": 8}, "too many"),
+    ({"blocks": 1 << 25}, "too many"), ({"q": FAKE.value + 8}, "16-byte aligned"), ({"k_row_stride": 66}, "16-byte aligned"),
+    ({"bf16": 1, "v_head_stride": 36}, "16-byte aligned"), ({"k": None}, "null"), ({"selected": None}, "null"),
+    ({"out": None}, "null"), (BIAS | {"axes": 4}, "1 to 3 axes"), (BIAS | {"buckets": 86}, "axes \\* buckets"),
+    (BIAS | {"reach": 683}, "reach"), (BIAS | {"reach": -1}, "1 to 3 axes"), (BIAS | {"map": None}, "map and cells"),
+    (BIAS | {"kv_heads": 1, "reach": 341}, "reach"),
+])
+def test_attend_argument_errors(changed, match):
+    L = _native.load()
+    args = _args(**changed)
+    n = ctypes.c_size_t(0)
+    for status in (L.tbvh_attend(ctypes.byref(args), None),
+                   L.tbvh_attend_backward_workspace_size(ctypes.byref(args), ctypes.byref(n)),
+                   L.tbvh_attend_backward(ctypes.byref(args), FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, 1 << 30, None)):
+        assert status == INVALID
+        with pytest.raises(AssertionError, match=match):
+            raise AssertionError(_err())
+
+
+def test_attend_backward_and_empty_calls():
+    L = _native.load()
+    assert L.tbvh_attend(None, None) == INVALID and "args is null" in _err()
+    assert L.tbvh_attend(ctypes.byref(_args(groups=0)), None) == 0
+    assert L.tbvh_attend(ctypes.byref(_args(q_rows=0)), None) == 0
+    args = _args()
+    n = ctypes.c_size_t(0)
+    assert L.tbvh_attend_backward_workspace_size(ctypes.byref(args), None) == INVALID
+    assert L.tbvh_attend_backward_workspace_size(ctypes.byref(args), ctypes.byref(n)) == 0 and n.value > 100 * 2 * 4
+
+    def backward(args, grad=FAKE, dq=FAKE, dtable=None, ws=FAKE, size=1 << 30):
+        return L.tbvh_attend_backward(ctypes.byref(args), grad, dq, FAKE, FAKE, dtable, ws, size, None)
+
+    assert backward(args, size=n.value - 1) == SMALL
+    for kw in ({"grad": None}, {"dq": None}, {"ws": None}, {"ws": ctypes.c_void_p(0x100010)},
+               {"grad": ctypes.c_void_p(0x100008)}):
+        assert backward(args, **kw) == INVALID
+    assert backward(_args(lse=None)) == INVALID
+    assert backward(_args(**BIAS)) == INVALID  # no dtable
+    for kw in ({"blocks": 0}, {"count": 0}, {"k_rows": 0}):
+        assert backward(_args(**kw)) == INVALID and "nothing to differentiate" in _err()
+
+
+def _norm(**changed):
+    a = dict(x=FAKE, offsets=None, rows=100, clouds=1, channels=8, groups=2, weight=FAKE, bias=FAKE, wide=0, bf16=0,
+             eps=1e-5, activation=2, y=FAKE, mean=FAKE, rstd=FAKE, ws=FAKE, ws_bytes=1 << 30, stream=None) | changed
+    return _native.load().tbvh_group_norm(*a.values())
+
+
+@pytest.mark.parametrize("changed,match", [
+    ({"rows": -1}, "rows >= 0"), ({"clouds": 0}, "65535 clouds"), ({"clouds": 65536}, "65535 clouds"),
+    ({"groups": 3}, "multiple of groups"), ({"groups": 0}, "multiple of groups"), ({"channels": 1 << 21}, "2\\^20"),
+    ({"rows": 1 << 40}, "2\\^40"), ({"clouds": 3}, "multiple of clouds"), ({"activation": 4}, "unknown activation"),
+    ({"activation": -1}, "unknown activation"), ({"eps": -1.0}, "eps"), ({"eps": float("nan")}, "eps"),
+    ({"x": None}, "null"), ({"y": None}, "null"), ({"mean": None}, "null"),
+    ({"ws": ctypes.c_void_p(0x100010)}, "aligned"), ({"ws": None}, "workspace is null"),
+])
+def test_norm_argument_errors(changed, match):
+    assert _norm(**changed) == INVALID
+    with pytest.raises(AssertionError, match=match):
+        raise AssertionError(_err())
+
+
+def test_norm_workspace_and_empty_calls():
+    L = _native.load()
+    assert _norm(ws_bytes=8) == SMALL
+    assert _norm(rows=0) == 0
+    n = ctypes.c_size_t(0)
+    assert L.tbvh_group_norm_workspace_size(1000, 2, 64, 8, ctypes.byref(n)) == 0 and n.value >= 2 * 64 * 2 * 4
+    assert L.tbvh_group_norm_workspace_size(1000, 2, 64, 8, None) == INVALID
+    a = [FAKE, FAKE, None, 0, 1, 8, 2, FAKE, FAKE, 0, 0, 1e-5, 2, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, 1 << 30, None]
+    assert L.tbvh_group_norm_backward(*a) == INVALID and "nothing to differentiate" in _err()
+    a[3], a[1] = 10, None
+    assert L.tbvh_group_norm_backward(*a) == INVALID and "null" in _err()

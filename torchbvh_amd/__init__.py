@@ -8,12 +8,22 @@ on first use and must have been built (``python -m torchbvh_amd._build``).
 
 import torch  # noqa: F401  (loads torch's HIP runtime before the native library)
 
+from ._blocks import (
+    BlockLayout,
+    RelativeBias,
+    block_attention,
+    block_boxes,
+    block_layout,
+    relative_buckets,
+    select_blocks,
+)
 from ._bvh_class import BVH
 from ._constants import SUPPORTED_DIMS, SUPPORTED_K
 from ._geometry import PointGeometry
 from ._handles import BVHHandle, BatchedBVHHandle, RaggedBVHHandle, destroy_bvh
 from ._multihead import gather_neighbor_values, interpolate_displaced, query_displaced_knn
 from ._native import _C
+from ._norm import group_norm_act
 from ._query import build_bvh, query_knn
 
 __version__ = "0.1.0"
@@ -30,6 +40,14 @@ __all__ = [
     "query_displaced_knn",
     "gather_neighbor_values",
     "interpolate_displaced",
+    "BlockLayout",
+    "RelativeBias",
+    "block_layout",
+    "block_boxes",
+    "select_blocks",
+    "relative_buckets",
+    "block_attention",
+    "group_norm_act",
     "SUPPORTED_K",
     "SUPPORTED_DIMS",
 ]

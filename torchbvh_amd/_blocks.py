@@ -1,0 +1,267 @@
+"""Attention between points, block by block.
+
+The rows of a call (points in the curve order of a BVH, their features) are
+packed cloud after cloud and cut into blocks of at most ``block_size`` rows that
+never straddle two clouds (`BlockLayout`).  With a power of two they are the
+nodes of one level of the tree, so a block's box is a node's (`block_boxes`).
+`select_blocks` chooses for every block of queries the key blocks nearest to it,
+`block_attention` attends to the chosen blocks' rows, with a learned bias of the
+relative position if wanted (`RelativeBias`).
+
+The reference has no counterpart.
+"""
+
+from __future__ import annotations
+
+import math
+from typing import NamedTuple
+
+import torch
+
+from ._constants import SUPPORTED_DIMS
+from ._handles import AnyHandle, BatchedBVHHandle, BVHHandle, RaggedBVHHandle, live_payload
+from ._native import _C
+from ._validation import check_cuda_f32, check_offsets, dense, dense_offsets
+
+__all__ = ["BlockLayout", "RelativeBias", "block_layout", "block_boxes", "block_attention", "relative_buckets",
+           "select_blocks"]
+
+MAX_BLOCK = 128      # rows of a block
+MAX_SELECTED = 64    # blocks that select_blocks chooses
+MAX_CHANNELS = 128   # channels of a head
+_TYPES = (torch.float32, torch.bfloat16)
+
+
+class BlockLayout(NamedTuple):
+    """How packed rows are cut into blocks (made, and checked, by
+    `block_layout`; a program keeps it as long as its clouds keep their sizes).
+
+    The entry points check the tensors' types and shapes, and the kernels read
+    no row outside a tensor whatever values the layout holds."""
+
+    offsets: torch.Tensor  # (clouds + 1,) int64: first row of each cloud
+    starts: torch.Tensor   # (blocks + 1,) int64: first row of each block
+    clouds: torch.Tensor   # (clouds + 1,) int64: first block of each cloud
+    block_size: int
+
+
+class RelativeBias(NamedTuple):
+    """A learned bias of the relative position: the sum over axes a of
+    ``table[a, buckets[clamp(query_cells[i, a] - key_cells[j, a], -R, R) + R], h]``
+    with ``R = len(buckets) // 2``.  Cells are whole numbers, such as
+    coordinates divided by a cell width, or positions in a sequence (one axis)."""
+
+    table: torch.Tensor        # (axes, buckets, heads), of the queries' type
+    buckets: torch.Tensor      # (2 R + 1,) int32, see `relative_buckets`
+    query_cells: torch.Tensor  # (query rows, axes) int32
+    key_cells: torch.Tensor    # (key rows, axes) int32
+
+
+def _refuse(op: str, *rules) -> None:
+    """ValueError for the first rule (holds, message) that does not hold."""
+    for holds, message in rules:
+        if not holds:
+            raise ValueError(f"{op}: {message}")
+
+
+def block_layout(source, block_size: int = 64, *, device=None) -> BlockLayout:
+    """The layout of a handle's points, of ``(B, N)`` equal clouds, or of packed
+    clouds given as ``(B + 1,)`` int64 CUDA offsets (read back to the host
+    once)."""
+    op = "block_layout"
+    _refuse(op, (isinstance(block_size, int) and 1 <= block_size <= MAX_BLOCK, f"block_size must be 1 to {MAX_BLOCK}"))
+    if isinstance(source, RaggedBVHHandle):
+        source = live_payload(source, RaggedBVHHandle, op)["batch_offsets"]
+    elif isinstance(source, (BVHHandle, BatchedBVHHandle)):
+        data = live_payload(source, type(source), op)
+        device = data["node_aabbs"].device
+        source = (data.get("batch_size", 1), data["num_leaves"])
+    if isinstance(source, torch.Tensor):
+        source = dense_offsets(source)
+        device = source.device
+        total = int(source[-1]) if source.dim() == 1 and source.numel() and source.dtype == torch.int64 else 0
+        offsets = check_offsets(op, source, total_rows=total, device=device)
+    else:
+        _refuse(op, (isinstance(source, tuple) and len(source) == 2, "source must be a handle, (B, N) or offsets"))
+        B, N = (int(x) for x in source)
+        _refuse(op, (B >= 1 and N >= 0, "need B >= 1 and N >= 0"))
+        offsets = list(range(0, B * N + 1, N)) if N else [0] * (B + 1)
+    device = torch.device("cuda") if device is None else torch.device(device)
+    bounds = torch.tensor(offsets, dtype=torch.int64)
+    counts = (bounds.diff() + block_size - 1).div(block_size, rounding_mode="floor")
+    clouds = torch.cat([counts.new_zeros(1), counts.cumsum(0)])
+    within = torch.arange(int(clouds[-1])) - clouds[:-1].repeat_interleave(counts)
+    starts = torch.cat([bounds[:-1].repeat_interleave(counts) + within * block_size, bounds[-1:]])
+    return BlockLayout(*(t.to(device) for t in (bounds, starts, clouds)), block_size)
+
+
+def block_boxes(bvh: AnyHandle, block_size: int = 64) -> torch.Tensor:
+    """The boxes ``(blocks, 2 D)`` (lower corner, upper corner) of the layout
+    that `block_layout` makes of a handle with the same ``block_size``, a power
+    of two: the tree's nodes over so many leaves."""
+    op = "block_boxes"
+    _refuse(op, (isinstance(block_size, int) and 1 <= block_size <= MAX_BLOCK and block_size & (block_size - 1) == 0,
+                 f"block_size must be a power of two up to {MAX_BLOCK}"))
+    if isinstance(bvh, RaggedBVHHandle):
+        live_payload(bvh, RaggedBVHHandle, op)
+        return torch.cat([block_boxes(h, block_size) for h in bvh._handles])
+    data = live_payload(bvh, BatchedBVHHandle if isinstance(bvh, BatchedBVHHandle) else BVHHandle, op)
+    n, dim = data["num_leaves"], data["dim"]
+    up = min(block_size.bit_length() - 1, data["leaf_level"])
+    level = data["leaf_level"] - up
+    # Virtual nodes above the level: 2 x - popcount(x), x of them one level up.
+    x = data["virtual_leaves"] >> (up + 1)
+    first = (1 << level) - 1 - (2 * x - bin(x).count("1"))
+    nodes = data["node_aabbs"]
+    return nodes[..., first : first + -(-n >> up), :].reshape(-1, 2 * dim).contiguous()
+
+
+def relative_buckets(sizes: int, max_distance: int, *, device=None) -> torch.Tensor:
+    """Bucket of every relative position from ``-max_distance`` to
+    ``max_distance`` as `RelativeBias` takes them: distances below ``sizes // 2``
+    have a bucket each, longer ones share ever wider ones, evenly in the logarithm up
+    to ``max_distance``.  Bucket 0 is distance zero, ``1 .. sizes - 1`` are
+    positive and ``sizes .. 2 sizes - 2`` negative distances, so a table needs
+    ``2 sizes - 1`` buckets."""
+    op = "relative_buckets"
+    _refuse(op, (sizes >= 2 and max_distance >= 1, "need sizes >= 2 and max_distance >= 1"))
+    near = max(sizes // 2, 1)
+
+    def size(d: int) -> int:
+        if d < near:
+            return d
+        reach = math.log(max(max_distance, near + 1) / near)
+        return min(near + int((sizes - near) * math.log(d / near) / reach), sizes - 1)
+
+    up = [size(d) for d in range(max_distance + 1)]
+    down = [sizes - 1 + b if b else 0 for b in up[:0:-1]]
+    return torch.tensor(down + up, dtype=torch.int32, device="cuda" if device is None else device)
+
+
+def _check_layout(op: str, layout: BlockLayout, name: str, device: torch.device) -> None:
+    ok = isinstance(layout, BlockLayout) and all(
+        isinstance(t, torch.Tensor) and t.dtype == torch.int64 and t.dim() == 1 and t.numel() >= 1 and t.is_contiguous()
+        for t in layout[:3])
+    _refuse(op, (ok and layout.offsets.numel() == layout.clouds.numel() >= 2 and 1 <= layout.block_size <= MAX_BLOCK,
+                 f"{name} must be a BlockLayout (see block_layout)"),
+            (ok and all(t.device == device for t in layout[:3]), f"{name} must be on the same device as the rows"))
+
+
+def select_blocks(queries: torch.Tensor, boxes: torch.Tensor, count: int, query_layout: BlockLayout,
+                  key_layout: BlockLayout) -> torch.Tensor:
+    """For every block of queries the ``count`` key blocks of the same cloud
+    whose boxes are nearest to the centre of the queries' box, as int32 block
+    numbers of ``key_layout`` in ascending (squared distance, block number),
+    -1 where the cloud has fewer.
+
+    ``queries (T, D)`` are packed like ``query_layout``; ``boxes (blocks, 2 D)``
+    come from `block_boxes`.  Query blocks of one row choose for each query.
+    Coordinates that are NaN are left out of a block's box; blocks at no finite
+    distance are not chosen."""
+    op = "select_blocks"
+    _refuse(op, (queries.dim() == 2, "queries must have shape (T, D)"),
+            (queries.dim() == 2 and queries.size(1) in SUPPORTED_DIMS, "D must be 2 or 3"))
+    check_cuda_f32(op, queries, "queries")
+    check_cuda_f32(op, boxes, "boxes")
+    _check_layout(op, query_layout, "query_layout", queries.device)
+    _check_layout(op, key_layout, "key_layout", queries.device)
+    _refuse(op, (boxes.dim() == 2 and boxes.size(1) == 2 * queries.size(1), "boxes must have shape (blocks, 2 D)"),
+            (boxes.device == queries.device, "boxes must be on the same device as queries"),
+            (boxes.size(0) == key_layout.starts.numel() - 1, "boxes must have a row for every block of key_layout"),
+            (query_layout.clouds.numel() == key_layout.clouds.numel(), "the layouts must have the same clouds"),
+            (1 <= count <= MAX_SELECTED, f"count must be 1 to {MAX_SELECTED}"))
+    return _C.select_blocks(dense(queries.detach()), query_layout.starts, query_layout.clouds, query_layout.block_size,
+                            dense(boxes.detach()), key_layout.clouds, int(count))
+
+
+def _rows_of(t: torch.Tensor) -> torch.Tensor:
+    """(rows, heads, D) whose channels are contiguous and whose rows and heads
+    start on 16 bytes: the tensor itself where it is so, as slices of one
+    projection of queries, keys and values are, else a copy."""
+    step = 16 // t.element_size()
+    ok = t.stride(2) == 1 and all(s % step == 0 for s in t.stride()[:2]) and t.data_ptr() % 16 == 0
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
+
+
+class _Attend(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, table, selected, query_layout, key_layout, scale, places):
+        q, k, v = _rows_of(q), _rows_of(k), _rows_of(v)
+        bias = None if table is None else (table, *places)
+        wanted = any(ctx.needs_input_grad[:4])
+        out, lse = _C.attend(q, k, v, selected, query_layout.starts, key_layout.starts, query_layout.block_size,
+                             key_layout.block_size, scale, bias, wanted)
+        if wanted:
+            ctx.save_for_backward(q, k, v, out, lse, table, selected, query_layout.starts, key_layout.starts,
+                                  *(places or ()))
+            ctx.sizes = (query_layout.block_size, key_layout.block_size, scale)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        q, k, v, out, lse, table, selected, q_starts, k_starts, *places = ctx.saved_tensors
+        if 0 in (q.numel(), k.numel(), selected.numel(), k_starts.numel() - 1):
+            grads = [torch.zeros_like(t) for t in (q, k, v)] + [None if table is None else torch.zeros_like(table)]
+        else:
+            bias = None if table is None else (table, *places)
+            grads = _C.attend_backward(_rows_of(grad.contiguous()), q, k, v, out, lse, selected, q_starts, k_starts,
+                                       *ctx.sizes, bias)
+        return *grads, None, None, None, None, None
+
+
+def block_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, selected: torch.Tensor,
+                    query_layout: BlockLayout, key_layout: BlockLayout, *, scale: float | None = None,
+                    bias: RelativeBias | None = None) -> torch.Tensor:
+    """Softmax attention of every row of ``q (rows, H, D)`` over the rows of
+    ``k``, ``v (rows, Hk, D)`` in the key blocks that ``selected`` holds for its
+    block: ``softmax(scale * q k^T + bias) v``, ``scale`` being ``D ** -0.5`` if not
+    given.  Differentiable in ``q``, ``k``, ``v`` and the bias's table, the same bits
+    on every call.
+
+    float32 or bfloat16, up to 128 channels (best a multiple of 8: others are
+    padded by a copy); ``H`` a multiple of ``Hk``, query head ``h`` reading
+    key head ``h // (H // Hk)``.  ``selected (query blocks, count)`` int32 comes from
+    `select_blocks` or any other choice; entries that are no block's number choose
+    nothing, a block chosen twice counts twice, and rows for which nothing is
+    chosen are zero."""
+    op = "block_attention"
+    _refuse(op, *((t.dim() == 3, f"{n} must have shape (rows, heads, D)") for n, t in (("q", q), ("k", k), ("v", v))))
+    _refuse(op, (q.is_cuda, "q must be a CUDA tensor"), (q.dtype in _TYPES, "q must be float32 or bfloat16"),
+            (k.dtype == q.dtype and v.dtype == q.dtype, "k and v must have q's type"),
+            (k.device == q.device and v.device == q.device, "k and v must be on the same device as q"),
+            (k.shape == v.shape, "k and v must have the same shape"),
+            (1 <= q.size(2) <= MAX_CHANNELS, f"D must be 1 to {MAX_CHANNELS}"),
+            (k.size(2) == q.size(2), "k and v must have q's channels"),
+            (k.size(1) >= 1 and q.size(1) >= 1 and q.size(1) % k.size(1) == 0,
+             "q's heads must be a multiple of k's"))
+    _check_layout(op, query_layout, "query_layout", q.device)
+    _check_layout(op, key_layout, "key_layout", q.device)
+    _refuse(op, (isinstance(selected, torch.Tensor) and selected.dim() == 2
+                 and selected.size(0) == query_layout.starts.numel() - 1,
+                 "selected must have shape (blocks of query_layout, count)"),
+            (selected.dtype == torch.int32, "selected must be int32"),
+            (selected.device == q.device, "selected must be on the same device as q"))
+    table = places = None
+    if bias is not None:
+        table, buckets, query_cells, key_cells = bias
+        _refuse(op, (table.dim() == 3 and 1 <= table.size(0) <= 3 and table.size(2) == q.size(1),
+                     "bias.table must have shape (axes, buckets, heads) with 1 to 3 axes and q's heads"),
+                (table.dtype == q.dtype, "bias.table must have q's type"),
+                (1 <= table.size(0) * table.size(1) <= 256, "bias.table must have at most 256 axes * buckets"),
+                (buckets.dim() == 1 and buckets.numel() % 2 == 1 and buckets.dtype == torch.int32,
+                 "bias.buckets must be int32 with an odd number of entries"),
+                (table.size(0) * buckets.numel() * (q.size(1) // k.size(1)) <= 4096,
+                 "bias.buckets must have at most 4096 / (axes * heads per key head) entries"),
+                *((t.dim() == 2 and tuple(t.shape) == (n, table.size(0)) and t.dtype == torch.int32,
+                   f"bias.{what} must be int32 of shape (rows, axes)")
+                  for what, t, n in (("query_cells", query_cells, q.size(0)), ("key_cells", key_cells, k.size(0)))),
+                *((t.device == q.device, "the bias must be on the same device as q")
+                  for t in (table, buckets, query_cells, key_cells)))
+        table, places = dense(table), tuple(dense(t.detach()) for t in (buckets, query_cells, key_cells))
+    D = q.size(2)
+    scale = D**-0.5 if scale is None else float(scale)
+    if D % 8:
+        q, k, v = (torch.nn.functional.pad(t, (0, -D % 8)) for t in (q, k, v))
+    out = _Attend.apply(q, k, v, table, dense(selected.detach()), query_layout, key_layout, scale, places)
+    return out[..., :D] if D % 8 else out

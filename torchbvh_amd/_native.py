@@ -40,6 +40,23 @@ _szp = ctypes.POINTER(ctypes.c_size_t)
 ABI_VERSION = 2
 
 
+class AttendArgs(ctypes.Structure):
+    """tbvh_attend_args of include/torchbvh_amd.h."""
+
+    _fields_ = (
+        [(n, _vp) for n in ("q", "k", "v")]
+        + [(n, _i64) for n in ("q_row_stride", "q_head_stride", "k_row_stride", "k_head_stride", "v_row_stride",
+                               "v_head_stride", "q_rows", "k_rows")]
+        + [(n, _vp) for n in ("selected", "q_starts", "k_starts")]
+        + [(n, _i64) for n in ("groups", "blocks")]
+        + [(n, ctypes.c_int32) for n in ("count", "q_block", "k_block", "heads", "kv_heads", "D", "bf16")]
+        + [("scale", ctypes.c_float)]
+        + [(n, _vp) for n in ("table", "map", "q_cells", "k_cells")]
+        + [(n, ctypes.c_int32) for n in ("axes", "buckets", "reach")]
+        + [(n, _vp) for n in ("out", "lse")]
+    )
+
+
 def _declare(L) -> None:
     L.tbvh_abi_version.restype = _int
     L.tbvh_last_error.restype = ctypes.c_char_p
@@ -149,7 +166,27 @@ def _declare(L) -> None:
     L.tbvh_interpolate_backward.argtypes = (
         [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _int, _vp, _vp, ctypes.c_size_t, _vp]
     )
+    L.tbvh_select_blocks_workspace_size.argtypes = [_i64, _int, _szp]
+    L.tbvh_select_blocks.argtypes = (
+        [_vp, _i64, _vp, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _int, _int, _vp, _vp, ctypes.c_size_t, _vp]
+    )
+    args = ctypes.POINTER(AttendArgs)
+    L.tbvh_attend.argtypes = [args, _vp]
+    L.tbvh_attend_backward_workspace_size.argtypes = [args, _szp]
+    L.tbvh_attend_backward.argtypes = [args] + [_vp] * 6 + [ctypes.c_size_t, _vp]
+    L.tbvh_group_norm_workspace_size.argtypes = [_i64, _i64, _i64, _i64, _szp]
+    L.tbvh_group_norm.argtypes = (
+        [_vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _int, _int, ctypes.c_float, _int, _vp, _vp, _vp, _vp,
+         ctypes.c_size_t, _vp]
+    )
+    L.tbvh_group_norm_backward.argtypes = (
+        [_vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _int, _int, ctypes.c_float, _int, _vp, _vp, _vp, _vp, _vp,
+         _vp, ctypes.c_size_t, _vp]
+    )
     for name in (
+        "tbvh_select_blocks_workspace_size", "tbvh_select_blocks", "tbvh_attend",
+        "tbvh_attend_backward_workspace_size", "tbvh_attend_backward", "tbvh_group_norm_workspace_size",
+        "tbvh_group_norm", "tbvh_group_norm_backward",
         "tbvh_build_workspace_size", "tbvh_build", "tbvh_build_ragged_workspace_size",
         "tbvh_build_ragged", "tbvh_build_with_accel", "tbvh_build_ragged_with_accel",
         "tbvh_sort_queries_workspace_size", "tbvh_sort_queries",
@@ -1197,6 +1234,147 @@ class _NativeOps:
                 _ptr(grad), _ptr(indices), _ptr(weights), _ptr(exact), B, N, H, C, k, _ptr(out), _ptr(ws),
                 ws.numel(), _stream(dev)))
         return out
+
+
+    @staticmethod
+    def select_blocks(queries, q_starts, q_clouds, q_block, boxes, k_clouds, count):
+        """Nearest blocks of every block of queries (`tbvh_select_blocks`):
+        int32 (groups, count)."""
+        op = "select_blocks"
+        _require_device_f32(op, queries, "queries")
+        _require_device_f32(op, boxes, "boxes")
+        for name, t in (("q_starts", q_starts), ("q_clouds", q_clouds), ("k_clouds", k_clouds)):
+            _require_device_i64(op, t, name)
+        dim, groups, blocks = int(queries.size(1)), int(q_starts.numel()) - 1, int(boxes.size(0))
+        dev = queries.device
+        out = torch.empty((groups, count), dtype=torch.int32, device=dev)
+        L = load()
+        with torch.cuda.device(dev):
+            ws = _workspace(_size(L.tbvh_select_blocks_workspace_size, blocks, dim), dev)
+            _check(L.tbvh_select_blocks(
+                _ptr(queries), queries.size(0), _ptr(q_starts), _ptr(q_clouds), groups, q_block, _ptr(boxes),
+                _ptr(k_clouds), blocks, q_clouds.numel() - 1, dim, count, _ptr(out), _ptr(ws), ws.numel(), _stream(dev)))
+        return out
+
+    @staticmethod
+    def attend(q, k, v, selected, q_starts, k_starts, q_block, k_block, scale, bias, want_lse):
+        """`tbvh_attend`: q (rows, heads, D), k and v (rows, kv_heads, D) with
+        contiguous channels; `bias` None or (table, map, q_cells, k_cells).
+        Returns the output and, if wanted, its log-sum-exp in base 2."""
+        args = _attend_args("attend", q, k, v, selected, q_starts, k_starts, q_block, k_block, scale, bias)
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if want_lse else None
+        args.out, args.lse = out.data_ptr(), None if lse is None else lse.data_ptr()
+        with torch.cuda.device(q.device):
+            _check(load().tbvh_attend(ctypes.byref(args), _stream(q.device)))
+        return out, lse
+
+    @staticmethod
+    def attend_backward(grad, q, k, v, out, lse, selected, q_starts, k_starts, q_block, k_block, scale, bias):
+        """`tbvh_attend_backward`: (dq, dk, dv, dtable or None)."""
+        op = "attend_backward"
+        _require(grad.shape == q.shape and grad.is_contiguous() and grad.dtype == q.dtype, op,
+                 "grad must be contiguous, of q's shape and type")
+        args = _attend_args(op, q, k, v, selected, q_starts, k_starts, q_block, k_block, scale, bias)
+        args.out, args.lse = out.data_ptr(), lse.data_ptr()
+        dev = q.device
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
+        dtable = None if bias is None else torch.empty(bias[0].shape, dtype=q.dtype, device=dev)
+        L = load()
+        with torch.cuda.device(dev):
+            ws = _workspace(_size(L.tbvh_attend_backward_workspace_size, ctypes.byref(args)), dev)
+            _check(L.tbvh_attend_backward(ctypes.byref(args), _ptr(grad), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dtable),
+                                          _ptr(ws), ws.numel(), _stream(dev)))
+        return dq, dk, dv, dtable
+
+    @staticmethod
+    def group_norm(x, offsets, clouds, groups, weight, bias, eps, activation):
+        """`tbvh_group_norm` of x (rows, channels): (y, mean, rstd)."""
+        op = "group_norm"
+        wide = _require_norm(op, x, offsets, weight, bias)
+        rows, channels = (int(n) for n in x.shape)
+        dev = x.device
+        y = torch.empty_like(x)
+        mean, rstd = (torch.empty((clouds, groups), dtype=torch.float32, device=dev) for _ in range(2))
+        L = load()
+        with torch.cuda.device(dev):
+            ws = _workspace(_size(L.tbvh_group_norm_workspace_size, rows, clouds, channels, groups), dev)
+            _check(L.tbvh_group_norm(_ptr(x), _ptr(offsets), rows, clouds, channels, groups, _ptr(weight), _ptr(bias),
+                                     wide, x.dtype == torch.bfloat16, eps, activation, _ptr(y), _ptr(mean), _ptr(rstd),
+                                     _ptr(ws), ws.numel(), _stream(dev)))
+        return y, mean, rstd
+
+    @staticmethod
+    def group_norm_backward(grad, x, offsets, clouds, groups, weight, bias, eps, activation, mean, rstd,
+                            want_dx, want_dweight, want_dbias):
+        """`tbvh_group_norm_backward`: (dx, dweight, dbias), None where not wanted."""
+        op = "group_norm_backward"
+        wide = _require_norm(op, x, offsets, weight, bias)
+        _require(grad.shape == x.shape and grad.is_contiguous() and grad.dtype == x.dtype, op,
+                 "grad must be contiguous, of x's shape and type")
+        rows, channels = (int(n) for n in x.shape)
+        dev = x.device
+        dx = torch.empty_like(x) if want_dx else None
+        dweight = torch.empty_like(weight) if want_dweight else None
+        dbias = torch.empty_like(bias) if want_dbias else None
+        L = load()
+        with torch.cuda.device(dev):
+            ws = _workspace(_size(L.tbvh_group_norm_workspace_size, rows, clouds, channels, groups), dev)
+            _check(L.tbvh_group_norm_backward(
+                _ptr(x), _ptr(grad), _ptr(offsets), rows, clouds, channels, groups, _ptr(weight), _ptr(bias), wide,
+                x.dtype == torch.bfloat16, eps, activation, _ptr(mean), _ptr(rstd), _ptr(dx), _ptr(dweight),
+                _ptr(dbias), _ptr(ws), ws.numel(), _stream(dev)))
+        return dx, dweight, dbias
+
+
+def _require_norm(op, x, offsets, weight, bias) -> bool:
+    """Checks a group norm's tensors; whether its parameters are fp32 beside a
+    narrower x."""
+    _require(x.is_cuda and x.is_contiguous() and x.dim() == 2 and x.dtype in (torch.float32, torch.bfloat16), op,
+             "x must be a contiguous CUDA tensor (rows, channels), float32 or bfloat16")
+    if offsets is not None:
+        _require_device_i64(op, offsets, "offsets")
+    given = [t for t in (weight, bias) if t is not None]
+    for t in given:
+        _require(t.device == x.device and t.is_contiguous() and tuple(t.shape) == (x.size(1),)
+                 and t.dtype == given[0].dtype and t.dtype in (x.dtype, torch.float32), op,
+                 "weight and bias must be contiguous (channels,) tensors of x's type or both float32, on x's device")
+    return bool(given) and given[0].dtype != x.dtype
+
+
+def _attend_args(op, q, k, v, selected, q_starts, k_starts, q_block, k_block, scale, bias) -> AttendArgs:
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        _require(t.is_cuda and t.device == q.device and t.dim() == 3 and t.dtype == q.dtype
+                 and t.dtype in (torch.float32, torch.bfloat16) and (t.stride(2) == 1 or t.numel() == 0), op,
+                 f"{name} must be a CUDA tensor (rows, heads, D) with contiguous channels, float32 or bfloat16 like q")
+    _require(k.shape == v.shape and k.size(2) == q.size(2), op, "k and v must have one shape, and q's channels")
+    for name, t in (("q_starts", q_starts), ("k_starts", k_starts)):
+        _require_device_i64(op, t, name)
+        _require(t.device == q.device and t.dim() == 1 and t.numel() >= 1, op, f"{name} must be (blocks + 1,) beside q")
+    groups = int(q_starts.numel()) - 1
+    _require(selected.is_cuda and selected.device == q.device and selected.dtype == torch.int32
+             and selected.is_contiguous() and selected.dim() == 2 and selected.size(0) == groups, op,
+             "selected must be a contiguous CUDA int32 tensor (groups, count)")
+    args = AttendArgs(
+        q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), q_row_stride=q.stride(0), q_head_stride=q.stride(1),
+        k_row_stride=k.stride(0), k_head_stride=k.stride(1), v_row_stride=v.stride(0), v_head_stride=v.stride(1),
+        q_rows=q.size(0), k_rows=k.size(0), selected=selected.data_ptr(), q_starts=q_starts.data_ptr(),
+        k_starts=k_starts.data_ptr(), groups=groups, blocks=int(k_starts.numel()) - 1, count=selected.size(1),
+        q_block=q_block, k_block=k_block, heads=q.size(1), kv_heads=k.size(1), D=q.size(2),
+        bf16=q.dtype == torch.bfloat16, scale=scale)
+    if bias is not None:
+        table, spread, q_cells, k_cells = bias
+        _require(table.is_contiguous() and table.dtype == q.dtype and table.dim() == 3 and table.size(2) == q.size(1)
+                 and table.device == q.device, op, "table must be a contiguous (axes, buckets, heads) tensor like q")
+        for name, t, shape in (("map", spread, None), ("q_cells", q_cells, (q.size(0), table.size(0))),
+                               ("k_cells", k_cells, (k.size(0), table.size(0)))):
+            _require(t.is_contiguous() and t.dtype == torch.int32 and t.device == q.device
+                     and (shape is None or tuple(t.shape) == shape), op, f"{name} must be a contiguous int32 tensor")
+        _require(spread.dim() == 1 and spread.numel() % 2 == 1, op, "map must hold an odd number of entries")
+        args.table, args.map = table.data_ptr(), spread.data_ptr()
+        args.q_cells, args.k_cells = q_cells.data_ptr(), k_cells.data_ptr()
+        args.axes, args.buckets, args.reach = table.size(0), table.size(1), int(spread.numel()) // 2
+    return args
 
 
 _C = _NativeOps()

@@ -1,0 +1,80 @@
+"""Group norm with an activation over channels-last features of point clouds.
+
+The reference has no counterpart.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from ._blocks import BlockLayout, _check_layout, _refuse
+from ._native import _C
+from ._validation import dense
+
+__all__ = ["group_norm_act"]
+
+# In the order of the native library's numbers.
+ACTIVATIONS = ("none", "relu", "silu", "gelu")
+
+
+class _GroupNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, offsets, clouds, groups, eps, activation):
+        y, mean, rstd = _C.group_norm(x, offsets, clouds, groups, weight, bias, eps, activation)
+        if any(ctx.needs_input_grad[:3]):
+            ctx.save_for_backward(x, weight, bias, offsets, mean, rstd)
+            ctx.sizes = (clouds, groups, eps, activation)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        x, weight, bias, offsets, mean, rstd = ctx.saved_tensors
+        clouds, groups, eps, activation = ctx.sizes
+        wanted = ctx.needs_input_grad[:3]
+        if x.numel() == 0:
+            grads = [torch.zeros_like(t) if w else None for t, w in zip((x, weight, bias), wanted)]
+        else:
+            grads = _C.group_norm_backward(dense(grad), x, offsets, clouds, groups, weight, bias, eps, activation,
+                                           mean, rstd, *wanted)
+        return *grads, None, None, None, None, None
+
+
+def group_norm_act(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None = None,
+                   bias: torch.Tensor | None = None, layout: BlockLayout | None = None, *, eps: float = 1e-5,
+                   activation: str = "silu") -> torch.Tensor:
+    """``act(weight * (x - mean) / sqrt(var + eps) + bias)`` with mean and
+    variance over a cloud's rows and each of ``num_groups`` groups of consecutive
+    channels; ``activation`` is "silu", "gelu" (by the error function), "relu" or
+    "none".  Differentiable in ``x``, ``weight`` and ``bias``, the same bits on every
+    call.
+
+    ``x`` is ``(N, C)`` or ``(B, N, C)``, or ``(total_N, C)`` packed like
+    ``layout``; float32 or bfloat16.  ``weight`` and ``bias (C,)`` are of its type or
+    float32."""
+    op = "group_norm_act"
+    _refuse(op, (x.dim() == 2 or (x.dim() == 3 and layout is None),
+                 "x must have shape (N, C) or (B, N, C), or (total_N, C) with a layout"),
+            (x.is_cuda, "x must be a CUDA tensor"),
+            (x.dtype in (torch.float32, torch.bfloat16), "x must be float32 or bfloat16"),
+            (num_groups >= 1 and x.size(-1) >= 1 and x.size(-1) % num_groups == 0,
+             "channels must be a multiple of num_groups"),
+            (activation in ACTIVATIONS, f"activation must be one of {', '.join(ACTIVATIONS)}"),
+            (eps >= 0.0, "eps must be >= 0"))
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None:
+            _refuse(op, (tuple(t.shape) == (x.size(-1),), f"{name} must have shape (C,)"),
+                    (t.dtype in (x.dtype, torch.float32), f"{name} must be float32 or of x's type"),
+                    (t.device == x.device, f"{name} must be on the same device as x"))
+    if weight is not None and bias is not None:
+        _refuse(op, (weight.dtype == bias.dtype, "weight and bias must have the same type"))
+    if layout is not None:
+        _check_layout(op, layout, "layout", x.device)
+    clouds = layout.offsets.numel() - 1 if layout is not None else x.size(0) if x.dim() == 3 else 1
+    if clouds == 0:
+        return torch.empty_like(x)
+    rows = dense(x).reshape(-1, x.size(-1))
+    y = _GroupNorm.apply(rows, None if weight is None else dense(weight), None if bias is None else dense(bias),
+                         None if layout is None else layout.offsets, clouds, num_groups, float(eps),
+                         ACTIVATIONS.index(activation))
+    return y.reshape(x.shape)

@@ -8,6 +8,8 @@
 #include <string>
 
 #include "../../include/torchbvh_amd.h"
+#include "attend.hpp"
+#include "norm.hpp"
 #include "tbvh_internal.hpp"
 
 using namespace tbvh;
@@ -1536,6 +1538,306 @@ int tbvh_interpolate_backward(const float* grad, const int64_t* indices, const f
     TBVH_TRY(op, launch_interpolate_backward(grad, indices, weights, exact, B, N, H, C, k, carve<Segment>(ws, l.sort.segs),
                                              l.sort.tiles, sb, carve<int64_t>(ws, l.order),
                                              carve<float>(ws, l.coef), out, static_cast<hipStream_t>(stream_ptr)));
+    return ok();
+}
+
+// ---- attention over blocks, group norm ----------------------------------------------
+
+namespace {
+constexpr int64_t kMaxGroups = int64_t{1} << 26;  // work-groups of 64 lanes that one launch holds
+
+bool multiple_of_16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+// Forward and backward alike: the kernels' arguments, after every size, stride
+// and pointer that they rely on has been looked at.
+int check_attend(const char* op, const tbvh_attend_args* x, AttendArgs& a) {
+    if (!x) return fail(TBVH_ERR_INVALID_ARGUMENT, "%s: args is null", op);
+    if (x->q_rows < 0 || x->k_rows < 0 || x->groups < 0 || x->blocks < 0 || x->groups >= kMaxRows ||
+        x->blocks >= kMaxRows || x->count < 0) {
+        return fail(TBVH_ERR_INVALID_ARGUMENT, "%s: rows, groups, blocks and count must be >= 0 and fit in int32", op);
+    }
+    if (x->heads < 1 || x->kv_heads < 1 || x->heads % x->kv_heads != 0) {
+        return fail(TBVH_ERR_INVALID_ARGUMENT, "%s: heads must be a positive multiple of kv_heads", op);
+    }
+    if (x->D < 8 || x->D > 128 || x->D % 8 != 0) {
+        return fail(TBVH_ERR_INVALID_ARGUMENT, "%s: D must be a multiple of 8 up to 128, got %d", op, x->D);
+    }
+    if (x->q_block < 1 || x->q_block > 128 || x->k_block < 1 || x->k_block > 128) {
+        return fail(TBVH_ERR_INVALID_ARGUMENT, "%s: blocks must hold 1 to 128 rows", op);
+    }
+    if (x->groups * std::max<int64_t>(x->count, 1) > kMaxRows) {
+        return fail(TBVH_ERR_INVALID_ARGUMENT, "%s: groups * count must fit in signed int32", op);
+    }
+    const int64_t share = x->heads / x->kv_heads;
+    // Tiles have 16 rows at least; the backward's, 32 of a key block.
+    if (x->groups * ((x->q_block * share + 15) / 16) > kMaxGroups / x->heads ||
+        x->blocks * 4 > kMaxGroups / x->heads) {
+        return fail(TBVH_ERR_INVALID_ARGUMENT, "%s: too many (block, head) pairs for one launch", op);
+    }
+    const int64_t strides = x->q_row_stride | x->q_head_stride | x->k_row_stride | x->k_head_stride | x->v_row_stride |
+                            x->v_head_stride;
+    if (strides * (x->bf16 ? 2 : 4) % 16 != 0 || !multiple_of_16(x->q) || !multiple_of_16(x->k) || !multiple_of_16(x->v) ||
+        !multiple_of_16(x->out)) {
+        return fail(TBVH_ERR_INVALID_ARGUMENT, "%s: q, k, v and out must be 16-byte aligned, and their strides", op);
+    }
+    if (x->table) {
+        if (x->axes < 1 || x->axes > 3 || x->buckets < 1 || x->reach < 0 || x->axes * int64_t{x->buckets} > kMaxBins ||
+            share * x->axes * (2 * int64_t{x->reach} + 1) > kMaxReachEntries) {
+            return fail(TBVH_ERR_INVALID_ARGUMENT,
+                        "%s: a bias needs 1 to 3 axes, axes * buckets <= %d and heads / kv_heads * axes * (2 reach + 1) "
+                        "<= %d", op, kMaxBins, kMaxReachEntries);
+        }
+        if (!x->map || !x->q_cells || !x->k_cells) {
+            return fail(TBVH_ERR_INVALID_ARGUMENT, "%s: a bias needs map and cells", op);
+        }
+    }
+    if (x->q_rows > 0 && x->groups > 0 &&
+        (!x->q || !x->out || !x->q_starts || (x->count > 0 && !x->selected) ||
+         (x->k_rows > 0 && x->blocks > 0 && (!x->k || !x->v || !x->k_starts)))) {
+        return fail(TBVH_ERR_INVALID_ARGUMENT, "%s: null input or output pointer", op);
+    }
+    a.q = x->q;
+    a.k = x->k;
+    a.v = x->v;
+    a.q_row = x->q_row_stride;
+    a.q_head = x->q_head_stride;
+    a.k_row = x->k_row_stride;
+    a.k_head = x->k_head_stride;
+    a.v_row = x->v_row_stride;
+    a.v_head = x->v_head_stride;
+    a.selected = x->selected;
+    a.q_starts = x->q_starts;
+    a.k_starts = x->k_starts;
+    a.q_total = x->q_rows;
+    a.k_total = x->k_rows;
+    a.groups = static_cast<int>(x->groups);
+    a.blocks = static_cast<int>(x->blocks);
+    a.count = x->count;
+    a.q_block = x->q_block;
+    a.k_block = x->k_block;
+    a.heads = x->heads;
+    a.kv_heads = x->kv_heads;
+    a.share = static_cast<int>(share);
+    a.D = x->D;
+    a.scale = x->scale;
+    a.table = x->table;
+    a.map = x->map;
+    a.q_cells = x->q_cells;
+    a.k_cells = x->k_cells;
+    a.axes = x->axes;
+    a.buckets = x->buckets;
+    a.reach = x->reach;
+    a.out = x->out;
+    a.lse = x->lse;
+    return TBVH_OK;
+}
+
+// The backward's scratch: the sort's, the sorted entries, each block's run, a dot
+// product per row and head, and the parts of the table's gradient.
+struct AttendLayout {
+    Layout sort;
+    size_t order = 0, runs = 0, delta = 0, table = 0, total = 0;
+    int64_t entries = 0;
+    int parts = 0;
+};
+AttendLayout make_attend_layout(const AttendArgs& a) {
+    AttendLayout l;
+    l.entries = static_cast<int64_t>(a.groups) * a.count;
+    if (l.entries > 0) l.sort = make_layout(1, l.entries, 3, false);
+    size_t at = l.sort.total;
+    l.order = at; at = align_up(at + static_cast<size_t>(l.entries) * 8);
+    l.runs = at; at = align_up(at + (static_cast<size_t>(a.blocks) + 1) * 4);
+    l.delta = at; at = align_up(at + static_cast<size_t>(a.q_total) * a.heads * 4);
+    l.parts = attend_table_parts(a.groups, a.q_block, a.heads);
+    l.table = at;
+    if (a.table) at = align_up(at + static_cast<size_t>(l.parts) * a.heads * a.axes * a.buckets * 4);
+    l.total = at;
+    return l;
+}
+
+// Sizes of a group norm.
+int check_norm(const char* op, int64_t rows, int64_t clouds, int64_t channels, int64_t groups) {
+    if (rows < 0 || clouds < 1 || clouds > 65535 || channels < 1 || groups < 1 || channels % groups != 0) {
+        return fail(TBVH_ERR_INVALID_ARGUMENT,
+                    "%s: need rows >= 0, 1 to 65535 clouds and channels a positive multiple of groups", op);
+    }
+    int64_t values = 0;
+    if (channels > (1 << 20) || __builtin_mul_overflow(rows, channels, &values) || values > (int64_t{1} << 40)) {
+        return fail(TBVH_ERR_INVALID_ARGUMENT, "%s: channels exceed 2^20 or rows * channels 2^40", op);
+    }
+    return TBVH_OK;
+}
+}  // namespace
+
+int tbvh_select_blocks_workspace_size(int64_t blocks, int D, size_t* bytes) {
+    const char* op = "tbvh_select_blocks_workspace_size";
+    if (!bytes) return fail(TBVH_ERR_INVALID_ARGUMENT, "%s: bytes is null", op);
+    if (int r = check_dim(op, D)) return r;
+    if (blocks < 0 || blocks >= kMaxRows) return fail(TBVH_ERR_INVALID_ARGUMENT, "%s: blocks must fit in int32", op);
+    *bytes = align_up(static_cast<size_t>((blocks + kWave - 1) / kWave) * 2 * D * sizeof(float));
+    return ok();
+}
+
+int tbvh_select_blocks(const float* queries, int64_t q_rows, const int64_t* q_starts, const int64_t* q_clouds,
+                       int64_t groups, int64_t q_block, const float* boxes, const int64_t* k_clouds, int64_t blocks,
+                       int64_t clouds, int D, int count, int32_t* out, void* ws, size_t ws_bytes, void* stream_ptr) {
+    const char* op = "tbvh_select_blocks";
+    if (int r = check_dim(op, D)) return r;
+    if (count < 1 || count > kWave) return fail(TBVH_ERR_INVALID_ARGUMENT, "%s: count must be 1 to 64", op);
+    if (q_block < 1 || q_block > 128) return fail(TBVH_ERR_INVALID_ARGUMENT, "%s: blocks must hold 1 to 128 rows", op);
+    if (q_rows < 0 || groups < 0 || groups > kMaxGroups || blocks < 0 || blocks >= kMaxRows || clouds < 1 ||
+        clouds >= kMaxRows) {
+        return fail(TBVH_ERR_INVALID_ARGUMENT, "%s: need 0 <= groups <= 2^26, blocks in int32 and clouds >= 1", op);
+    }
+    if (groups == 0) return ok();
+    if (!q_starts || !q_clouds || !k_clouds || !out || (q_rows > 0 && !queries) || (blocks > 0 && !boxes)) {
+        return fail(TBVH_ERR_INVALID_ARGUMENT, "%s: null input or output pointer", op);
+    }
+    const size_t need = align_up(static_cast<size_t>((blocks + kWave - 1) / kWave) * 2 * D * sizeof(float));
+    if (int r = check_workspace(op, ws, ws_bytes, need)) return r;
+    SelectArgs a;
+    a.queries = queries;
+    a.boxes = boxes;
+    a.q_starts = q_starts;
+    a.q_clouds = q_clouds;
+    a.k_clouds = k_clouds;
+    a.q_total = q_rows;
+    a.groups = static_cast<int>(groups);
+    a.blocks = static_cast<int>(blocks);
+    a.clouds = static_cast<int>(clouds);
+    a.q_block = static_cast<int>(q_block);
+    a.count = count;
+    a.coarse = static_cast<float*>(ws);
+    a.out = out;
+    TBVH_TRY(op, launch_select(a, D, static_cast<hipStream_t>(stream_ptr)));
+    return ok();
+}
+
+int tbvh_attend(const tbvh_attend_args* args, void* stream_ptr) {
+    const char* op = "tbvh_attend";
+    AttendArgs a;
+    if (int r = check_attend(op, args, a)) return r;
+    if (a.groups == 0 || a.q_total == 0) return ok();
+    TBVH_TRY(op, launch_attend(a, args->bf16 != 0, static_cast<hipStream_t>(stream_ptr)));
+    return ok();
+}
+
+int tbvh_attend_backward_workspace_size(const tbvh_attend_args* args, size_t* bytes) {
+    const char* op = "tbvh_attend_backward_workspace_size";
+    if (!bytes) return fail(TBVH_ERR_INVALID_ARGUMENT, "%s: bytes is null", op);
+    AttendArgs a;
+    if (int r = check_attend(op, args, a)) return r;
+    *bytes = make_attend_layout(a).total;
+    return ok();
+}
+
+int tbvh_attend_backward(const tbvh_attend_args* args, const void* grad, void* dq, void* dk, void* dv, void* dtable,
+                         void* ws, size_t ws_bytes, void* stream_ptr) {
+    const char* op = "tbvh_attend_backward";
+    AttendArgs a;
+    if (int r = check_attend(op, args, a)) return r;
+    if (a.groups == 0 || a.blocks == 0 || a.q_total == 0 || a.k_total == 0 || a.count == 0) {
+        return fail(TBVH_ERR_INVALID_ARGUMENT, "%s: nothing to differentiate", op);
+    }
+    if (!grad || !dq || !dk || !dv || !a.lse || (a.table && !dtable)) {
+        return fail(TBVH_ERR_INVALID_ARGUMENT, "%s: null input or output pointer", op);
+    }
+    if (!multiple_of_16(grad) || !multiple_of_16(dq) || !multiple_of_16(dk) || !multiple_of_16(dv)) {
+        return fail(TBVH_ERR_INVALID_ARGUMENT, "%s: gradients must be 16-byte aligned", op);
+    }
+    const AttendLayout l = make_attend_layout(a);
+    if (int r = check_workspace(op, ws, ws_bytes, l.total)) return r;
+    const hipStream_t stream = static_cast<hipStream_t>(stream_ptr);
+    SortBuffers sb = sort_buffers(ws, l.sort);
+    sb.tstride = sort_tstride(l.entries, sb.tstride);
+    AttendGrads g;
+    g.grad = grad;
+    g.delta = carve<float>(ws, l.delta);
+    g.order = carve<int64_t>(ws, l.order);
+    g.runs = carve<int32_t>(ws, l.runs);
+    g.dq = dq;
+    g.dk = dk;
+    g.dv = dv;
+    g.dtable = dtable;
+    g.table_parts = carve<float>(ws, l.table);
+    g.parts = l.parts;
+    TBVH_TRY(op, launch_invert(a.selected, l.entries, a.blocks, carve<Segment>(ws, l.sort.segs), l.sort.tiles, sb,
+                               carve<int64_t>(ws, l.order), carve<int32_t>(ws, l.runs), stream));
+    TBVH_TRY(op, launch_attend_backward(a, g, args->bf16 != 0, stream));
+    return ok();
+}
+
+int tbvh_group_norm_workspace_size(int64_t rows, int64_t clouds, int64_t channels, int64_t groups, size_t* bytes) {
+    const char* op = "tbvh_group_norm_workspace_size";
+    if (!bytes) return fail(TBVH_ERR_INVALID_ARGUMENT, "%s: bytes is null", op);
+    if (int r = check_norm(op, rows, clouds, channels, groups)) return r;
+    *bytes = align_up(static_cast<size_t>(norm_scratch(rows, static_cast<int>(clouds), static_cast<int>(channels),
+                                                       static_cast<int>(groups))) * sizeof(float));
+    return ok();
+}
+
+namespace {
+// The part of the two entry points that they share.
+int fill_norm(const char* op, NormArgs& a, const void* x, const int64_t* offsets, int64_t rows, int64_t clouds,
+              int64_t channels, int64_t groups, const void* weight, const void* bias, float eps, int activation,
+              void* ws, size_t ws_bytes) {
+    if (int r = check_norm(op, rows, clouds, channels, groups)) return r;
+    if (!offsets && rows % clouds != 0) {
+        return fail(TBVH_ERR_INVALID_ARGUMENT, "%s: rows must be a multiple of clouds without offsets", op);
+    }
+    if (activation < kNone || activation > kGelu) return fail(TBVH_ERR_INVALID_ARGUMENT, "%s: unknown activation", op);
+    if (!(eps >= 0.0f)) return fail(TBVH_ERR_INVALID_ARGUMENT, "%s: eps must be >= 0", op);
+    const size_t need = static_cast<size_t>(norm_scratch(rows, static_cast<int>(clouds), static_cast<int>(channels),
+                                                         static_cast<int>(groups))) * sizeof(float);
+    if (int r = check_workspace(op, ws, ws_bytes, need)) return r;
+    a.x = x;
+    a.offsets = offsets;
+    a.rows = rows;
+    a.clouds = static_cast<int>(clouds);
+    a.channels = static_cast<int>(channels);
+    a.groups = static_cast<int>(groups);
+    a.weight = weight;
+    a.bias = bias;
+    a.eps = eps;
+    a.activation = activation;
+    a.parts = static_cast<float*>(ws);
+    return TBVH_OK;
+}
+}  // namespace
+
+int tbvh_group_norm(const void* x, const int64_t* offsets, int64_t rows, int64_t clouds, int64_t channels,
+                    int64_t groups, const void* weight, const void* bias, int wide_weights, int bf16, float eps,
+                    int activation, void* y, float* mean, float* rstd, void* ws, size_t ws_bytes, void* stream_ptr) {
+    const char* op = "tbvh_group_norm";
+    NormArgs a;
+    if (int r = fill_norm(op, a, x, offsets, rows, clouds, channels, groups, weight, bias, eps, activation, ws, ws_bytes))
+        return r;
+    if (rows == 0) return ok();
+    if (!x || !y || !mean || !rstd) return fail(TBVH_ERR_INVALID_ARGUMENT, "%s: null input or output pointer", op);
+    a.y = y;
+    a.mean = mean;
+    a.rstd = rstd;
+    TBVH_TRY(op, launch_norm(a, bf16 != 0, wide_weights != 0, static_cast<hipStream_t>(stream_ptr)));
+    return ok();
+}
+
+int tbvh_group_norm_backward(const void* x, const void* grad, const int64_t* offsets, int64_t rows, int64_t clouds,
+                             int64_t channels, int64_t groups, const void* weight, const void* bias, int wide_weights,
+                             int bf16, float eps, int activation, const float* mean, const float* rstd, void* dx,
+                             void* dweight, void* dbias, void* ws, size_t ws_bytes, void* stream_ptr) {
+    const char* op = "tbvh_group_norm_backward";
+    NormArgs a;
+    if (int r = fill_norm(op, a, x, offsets, rows, clouds, channels, groups, weight, bias, eps, activation, ws, ws_bytes))
+        return r;
+    if (rows == 0) return fail(TBVH_ERR_INVALID_ARGUMENT, "%s: nothing to differentiate", op);
+    if (!x || !grad || !mean || !rstd) return fail(TBVH_ERR_INVALID_ARGUMENT, "%s: null input or output pointer", op);
+    a.grad = grad;
+    a.mean = const_cast<float*>(mean);
+    a.rstd = const_cast<float*>(rstd);
+    a.dx = dx;
+    a.dweight = dweight;
+    a.dbias = dbias;
+    TBVH_TRY(op, launch_norm_backward(a, bf16 != 0, wide_weights != 0, static_cast<hipStream_t>(stream_ptr)));
     return ok();
 }
 

@@ -1,0 +1,432 @@
+// Group norm with an activation, rows of channels (channels last), statistics
+// over a cloud's rows and a group's channels:
+//
+//   xhat = (x - mean) rstd,  z = w xhat + b,  y = act(z)
+//   dz = dy act'(z),  dw = sum dz xhat,  db = sum dz
+//   dx = rstd (w dz - mean(w dz) - xhat mean(w dz xhat))
+//
+// Forward: a launch that leaves every slice's mean and sum of squared deviations
+// of each channel, one that joins them, one that writes y.  Backward: the same
+// shape around the two sums per channel.  All sums are fp32 in a fixed order;
+// squares are summed around means (of eight rows, then of a thread's, then joined
+// by n, mean and squares), so a large mean costs no digits.
+#include "norm.hpp"
+
+namespace tbvh {
+namespace {
+
+using bf16x8 = __bf16 __attribute__((ext_vector_type(8)));
+using f32x4 = float __attribute__((ext_vector_type(4)));
+
+template <typename T, int V>
+struct Vec {
+    T v[V];
+} __attribute__((aligned(sizeof(T) * V)));
+
+// Rows [first, last) of slice `part` of `parts` of a cloud.
+struct Slice {
+    int64_t first, last, cloud_rows;
+};
+__device__ __forceinline__ Slice slice_of(const NormArgs& a, int cloud, int part, int parts) {
+    int64_t lo = a.rows / a.clouds * cloud, hi = lo + a.rows / a.clouds;
+    if (a.offsets != nullptr) {
+        lo = min(max(a.offsets[cloud], int64_t{0}), a.rows);
+        hi = min(max(a.offsets[cloud + 1], lo), a.rows);
+    }
+    const int64_t n = hi - lo, each = (n + parts - 1) / parts;
+    const int64_t first = min(lo + each * part, hi);
+    return {first, min(first + each, hi), n};
+}
+
+// (n, mean, squares) of two disjoint sets of values.
+struct Moments {
+    float n, mean, squares;
+};
+__device__ __forceinline__ Moments join(Moments a, Moments b) {
+    const float n = a.n + b.n;
+    if (n == 0.0f) return a;
+    const float f = b.n / n, d = b.mean - a.mean;
+    return {n, a.mean + d * f, a.squares + b.squares + d * d * a.n * f};
+}
+
+template <int kAct>
+__device__ __forceinline__ float activate(float z) {
+    if constexpr (kAct == kRelu) return fmaxf(z, 0.0f);
+    if constexpr (kAct == kSilu) return z / (1.0f + __expf(-z));
+    if constexpr (kAct == kGelu) return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+    return z;
+}
+template <int kAct>
+__device__ __forceinline__ float slope(float z) {
+    if constexpr (kAct == kRelu) return z > 0.0f ? 1.0f : 0.0f;
+    if constexpr (kAct == kSilu) {
+        const float s = 1.0f / (1.0f + __expf(-z));
+        return s * (1.0f + z * (1.0f - s));
+    }
+    if constexpr (kAct == kGelu) {
+        return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * 0.39894228040143268f * __expf(-0.5f * z * z);
+    }
+    return 1.0f;
+}
+
+// A work-group of kBlock threads covers a strip of at most kBlock vectors of V
+// channels, and as many rows at once as fit: thread t takes vector t % strip of
+// rows t / strip, t / strip + step, ...
+struct Place {
+    int strip, step, column, row;  // column: first channel; row < 0: idle
+};
+template <int V>
+__device__ __forceinline__ Place place(int channels) {
+    const int vectors = channels / V - static_cast<int>(blockIdx.z) * kBlock;
+    const int strip = min(vectors, kBlock), step = kBlock / strip;
+    const int t = static_cast<int>(threadIdx.x), row = t / strip;
+    return {strip, step, (static_cast<int>(blockIdx.z) * kBlock + t - row * strip) * V, row < step ? row : -1};
+}
+
+constexpr int kRowsAtOnce = 8;
+
+// parts: (cloud, part, channel) -> (mean, squares).
+template <typename T, int V>
+__global__ __launch_bounds__(kBlock) void norm_stats_kernel(NormArgs a) {
+    __shared__ float s_mean[kBlock * V], s_squares[kBlock * V], s_n[kBlock];
+    const Place p = place<V>(a.channels);
+    const int cloud = blockIdx.y, part = blockIdx.x, parts = gridDim.x;
+    const Slice s = slice_of(a, cloud, part, parts);
+    Moments m[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) m[i] = {0.0f, 0.0f, 0.0f};
+    const T* x = static_cast<const T*>(a.x) + p.column;
+    if (p.row >= 0) {
+        for (int64_t r = s.first + p.row; r < s.last; r += static_cast<int64_t>(p.step) * kRowsAtOnce) {
+            Vec<T, V> v[kRowsAtOnce];
+            int n = 0;
+#pragma unroll
+            for (int j = 0; j < kRowsAtOnce; ++j) {
+                const int64_t row = r + static_cast<int64_t>(j) * p.step;
+                if (row < s.last) {
+                    v[j] = *reinterpret_cast<const Vec<T, V>*>(x + row * a.channels);
+                    ++n;
+                }
+            }
+            const float inverse = 1.0f / static_cast<float>(n);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                float sum = 0.0f, squares = 0.0f;
+#pragma unroll
+                for (int j = 0; j < kRowsAtOnce; ++j) sum += j < n ? static_cast<float>(v[j].v[i]) : 0.0f;
+                const float mean = sum * inverse;
+#pragma unroll
+                for (int j = 0; j < kRowsAtOnce; ++j) {
+                    const float d = j < n ? static_cast<float>(v[j].v[i]) - mean : 0.0f;
+                    squares = __builtin_fmaf(d, d, squares);
+                }
+                m[i] = join(m[i], {static_cast<float>(n), mean, squares});
+            }
+        }
+    }
+    s_n[threadIdx.x] = m[0].n;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        s_mean[threadIdx.x * V + i] = m[i].mean;
+        s_squares[threadIdx.x * V + i] = m[i].squares;
+    }
+    __syncthreads();
+    // Channel c of the strip: its threads' moments in row order.
+    const int first = static_cast<int>(blockIdx.z) * kBlock * V;
+    float* out = a.parts + (static_cast<int64_t>(cloud) * parts + part) * a.channels * 2;
+    for (int c = threadIdx.x; c < p.strip * V; c += kBlock) {
+        Moments sum = {0.0f, 0.0f, 0.0f};
+        for (int r = 0; r < p.step; ++r) {
+            const int t = r * p.strip + c / V;
+            sum = join(sum, {s_n[t], s_mean[t * V + c % V], s_squares[t * V + c % V]});
+        }
+        out[(first + c) * 2] = sum.mean;
+        out[(first + c) * 2 + 1] = sum.squares;
+    }
+}
+
+__device__ __forceinline__ Moments join_across(Moments m) {
+#pragma unroll
+    for (int d = 1; d < kWave; d <<= 1) {
+        const Moments o = {__shfl_xor(m.n, d, kWave), __shfl_xor(m.mean, d, kWave), __shfl_xor(m.squares, d, kWave)};
+        // Both lanes of a pair join in the same order.
+        m = lane_id() & d ? join(o, m) : join(m, o);
+    }
+    return m;
+}
+
+// One work-group per (group, cloud): the slices' moments of the group's channels.
+__global__ __launch_bounds__(kBlock) void norm_join_kernel(NormArgs a, int parts) {
+    __shared__ Moments s_m[kBlock / kWave];
+    const int cloud = blockIdx.y, group = blockIdx.x, per = a.channels / a.groups;
+    const float* in = a.parts + static_cast<int64_t>(cloud) * parts * a.channels * 2;
+    Moments m = {0.0f, 0.0f, 0.0f};
+    for (int i = threadIdx.x; i < parts * per; i += kBlock) {
+        const int part = i / per, c = group * per + i - part * per;
+        const Slice s = slice_of(a, cloud, part, parts);
+        const float* p = in + (static_cast<int64_t>(part) * a.channels + c) * 2;
+        m = join(m, {static_cast<float>(s.last - s.first), p[0], p[1]});
+    }
+    m = join_across(m);
+    if (lane_id() == 0) s_m[threadIdx.x / kWave] = m;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        m = s_m[0];
+        for (int w = 1; w < kBlock / kWave; ++w) m = join(m, s_m[w]);
+        a.mean[cloud * a.groups + group] = m.mean;
+        a.rstd[cloud * a.groups + group] = m.n > 0.0f ? 1.0f / sqrtf(m.squares / m.n + a.eps) : 0.0f;
+    }
+}
+
+// A thread's channels: z = (x - mean) scale + shift.
+template <typename P, int V>
+struct Columns {
+    float mean[V], rstd[V], weight[V], bias[V];
+    __device__ __forceinline__ void load(const NormArgs& a, int cloud, int column) {
+        const int per = a.channels / a.groups;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int at = cloud * a.groups + (column + i) / per;
+            mean[i] = a.mean[at];
+            rstd[i] = a.rstd[at];
+            weight[i] = a.weight ? static_cast<float>(static_cast<const P*>(a.weight)[column + i]) : 1.0f;
+            bias[i] = a.bias ? static_cast<float>(static_cast<const P*>(a.bias)[column + i]) : 0.0f;
+        }
+    }
+};
+
+template <typename T, typename P, int V, int kAct>
+__global__ __launch_bounds__(kBlock) void norm_apply_kernel(NormArgs a) {
+    const Place p = place<V>(a.channels);
+    if (p.row < 0) return;
+    const Slice s = slice_of(a, blockIdx.y, blockIdx.x, gridDim.x);
+    Columns<P, V> c;
+    c.load(a, blockIdx.y, p.column);
+    const T* x = static_cast<const T*>(a.x) + p.column;
+    T* y = static_cast<T*>(a.y) + p.column;
+    for (int64_t r = s.first + p.row; r < s.last; r += p.step) {
+        const Vec<T, V> v = *reinterpret_cast<const Vec<T, V>*>(x + r * a.channels);
+        Vec<T, V> o;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const float hat = (static_cast<float>(v.v[i]) - c.mean[i]) * c.rstd[i];
+            o.v[i] = static_cast<T>(activate<kAct>(__builtin_fmaf(hat, c.weight[i], c.bias[i])));
+        }
+        *reinterpret_cast<Vec<T, V>*>(y + r * a.channels) = o;
+    }
+}
+
+// parts: (cloud, part, channel) -> (sum dz, sum dz xhat).
+template <typename T, typename P, int V, int kAct>
+__global__ __launch_bounds__(kBlock) void norm_sums_kernel(NormArgs a) {
+    __shared__ float s_sum[kBlock * V], s_hat[kBlock * V];
+    const Place p = place<V>(a.channels);
+    const int cloud = blockIdx.y, part = blockIdx.x, parts = gridDim.x;
+    const Slice s = slice_of(a, cloud, part, parts);
+    float sum[V], hats[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) sum[i] = hats[i] = 0.0f;
+    if (p.row >= 0) {
+        Columns<P, V> c;
+        c.load(a, cloud, p.column);
+        const T* x = static_cast<const T*>(a.x) + p.column;
+        const T* up = static_cast<const T*>(a.grad) + p.column;
+        for (int64_t r = s.first + p.row; r < s.last; r += p.step) {
+            const Vec<T, V> v = *reinterpret_cast<const Vec<T, V>*>(x + r * a.channels);
+            const Vec<T, V> u = *reinterpret_cast<const Vec<T, V>*>(up + r * a.channels);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float hat = (static_cast<float>(v.v[i]) - c.mean[i]) * c.rstd[i];
+                const float dz = static_cast<float>(u.v[i]) * slope<kAct>(__builtin_fmaf(hat, c.weight[i], c.bias[i]));
+                sum[i] += dz;
+                hats[i] = __builtin_fmaf(dz, hat, hats[i]);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        s_sum[threadIdx.x * V + i] = sum[i];
+        s_hat[threadIdx.x * V + i] = hats[i];
+    }
+    __syncthreads();
+    const int first = static_cast<int>(blockIdx.z) * kBlock * V;
+    float* out = a.parts + (static_cast<int64_t>(cloud) * parts + part) * a.channels * 2;
+    for (int k = threadIdx.x; k < p.strip * V; k += kBlock) {
+        float x = 0.0f, y = 0.0f;
+        for (int r = 0; r < p.step; ++r) {
+            const int t = r * p.strip + k / V;
+            x += s_sum[t * V + k % V];
+            y += s_hat[t * V + k % V];
+        }
+        out[(first + k) * 2] = x;
+        out[(first + k) * 2 + 1] = y;
+    }
+}
+
+// One wave per (channel, cloud): the slices' sums, into `channel_sums`
+// (cloud, channel) -> (sum dz, sum dz xhat).
+__global__ __launch_bounds__(kWave) void norm_channel_kernel(NormArgs a, int parts, float* __restrict__ channel_sums) {
+    const int c = blockIdx.x, cloud = blockIdx.y;
+    float x = 0.0f, y = 0.0f;
+    for (int i = lane_id(); i < parts; i += kWave) {
+        const float* p = a.parts + ((static_cast<int64_t>(cloud) * parts + i) * a.channels + c) * 2;
+        x += p[0];
+        y += p[1];
+    }
+#pragma unroll
+    for (int d = kWave / 2; d > 0; d >>= 1) {
+        x += __shfl_xor(x, d, kWave);
+        y += __shfl_xor(y, d, kWave);
+    }
+    if (lane_id() == 0) {
+        channel_sums[(static_cast<int64_t>(cloud) * a.channels + c) * 2] = x;
+        channel_sums[(static_cast<int64_t>(cloud) * a.channels + c) * 2 + 1] = y;
+    }
+}
+
+// One wave per channel: the clouds' sums are the parameters' gradients.
+template <typename P>
+__global__ __launch_bounds__(kWave) void norm_weights_kernel(NormArgs a, const float* __restrict__ channel_sums) {
+    const int c = blockIdx.x;
+    float x = 0.0f, y = 0.0f;
+    for (int i = lane_id(); i < a.clouds; i += kWave) {
+        x += channel_sums[(static_cast<int64_t>(i) * a.channels + c) * 2];
+        y += channel_sums[(static_cast<int64_t>(i) * a.channels + c) * 2 + 1];
+    }
+#pragma unroll
+    for (int d = kWave / 2; d > 0; d >>= 1) {
+        x += __shfl_xor(x, d, kWave);
+        y += __shfl_xor(y, d, kWave);
+    }
+    if (lane_id() == 0) {
+        if (a.dbias) static_cast<P*>(a.dbias)[c] = static_cast<P>(x);
+        if (a.dweight) static_cast<P*>(a.dweight)[c] = static_cast<P>(y);
+    }
+}
+
+template <typename T, typename P, int V, int kAct>
+__global__ __launch_bounds__(kBlock) void norm_dx_kernel(NormArgs a, const float* __restrict__ channel_sums) {
+    const Place p = place<V>(a.channels);
+    if (p.row < 0) return;
+    const int cloud = blockIdx.y;
+    const Slice s = slice_of(a, cloud, blockIdx.x, gridDim.x);
+    if (s.first + p.row >= s.last) return;
+    Columns<P, V> c;
+    c.load(a, cloud, p.column);
+    // The group's means of w dz and w dz xhat, from its channels' sums.
+    const int per = a.channels / a.groups;
+    const float inverse = 1.0f / (static_cast<float>(s.cloud_rows) * static_cast<float>(per));
+    float mean[V], hats[V];
+    int known = -1;
+    float gm = 0.0f, gh = 0.0f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int group = (p.column + i) / per;
+        if (group != known) {
+            known = group;
+            gm = gh = 0.0f;
+            for (int k = group * per; k < (group + 1) * per; ++k) {
+                const float w = a.weight ? static_cast<float>(static_cast<const P*>(a.weight)[k]) : 1.0f;
+                gm = __builtin_fmaf(w, channel_sums[(static_cast<int64_t>(cloud) * a.channels + k) * 2], gm);
+                gh = __builtin_fmaf(w, channel_sums[(static_cast<int64_t>(cloud) * a.channels + k) * 2 + 1], gh);
+            }
+            gm *= inverse;
+            gh *= inverse;
+        }
+        mean[i] = gm;
+        hats[i] = gh;
+    }
+    const T* x = static_cast<const T*>(a.x) + p.column;
+    const T* up = static_cast<const T*>(a.grad) + p.column;
+    T* dx = static_cast<T*>(a.dx) + p.column;
+    for (int64_t r = s.first + p.row; r < s.last; r += p.step) {
+        const Vec<T, V> v = *reinterpret_cast<const Vec<T, V>*>(x + r * a.channels);
+        const Vec<T, V> u = *reinterpret_cast<const Vec<T, V>*>(up + r * a.channels);
+        Vec<T, V> o;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const float hat = (static_cast<float>(v.v[i]) - c.mean[i]) * c.rstd[i];
+            const float dz = static_cast<float>(u.v[i]) * slope<kAct>(__builtin_fmaf(hat, c.weight[i], c.bias[i]));
+            o.v[i] = static_cast<T>(c.rstd[i] * (c.weight[i] * dz - mean[i] - hat * hats[i]));
+        }
+        *reinterpret_cast<Vec<T, V>*>(dx + r * a.channels) = o;
+    }
+}
+
+dim3 strips(const NormArgs& a, int V, int parts) {
+    return dim3(static_cast<unsigned>(parts), static_cast<unsigned>(a.clouds),
+                static_cast<unsigned>((a.channels / V + kBlock - 1) / kBlock));
+}
+
+template <typename T, typename P, int V, int kAct>
+hipError_t run_forward(const NormArgs& a, hipStream_t stream) {
+    const int parts = norm_parts(a.rows, a.clouds, a.channels);
+    const dim3 grid = strips(a, V, parts);
+    norm_stats_kernel<T, V><<<grid, kBlock, 0, stream>>>(a);
+    norm_join_kernel<<<dim3(a.groups, a.clouds), kBlock, 0, stream>>>(a, parts);
+    norm_apply_kernel<T, P, V, kAct><<<grid, kBlock, 0, stream>>>(a);
+    return hipGetLastError();
+}
+
+template <typename T, typename P, int V, int kAct>
+hipError_t run_backward(const NormArgs& a, hipStream_t stream) {
+    const int parts = norm_parts(a.rows, a.clouds, a.channels);
+    const dim3 grid = strips(a, V, parts);
+    float* channel_sums = a.parts + static_cast<int64_t>(a.clouds) * parts * a.channels * 2;
+    norm_sums_kernel<T, P, V, kAct><<<grid, kBlock, 0, stream>>>(a);
+    norm_channel_kernel<<<dim3(a.channels, a.clouds), kWave, 0, stream>>>(a, parts, channel_sums);
+    if (a.dweight || a.dbias) norm_weights_kernel<P><<<a.channels, kWave, 0, stream>>>(a, channel_sums);
+    if (a.dx) norm_dx_kernel<T, P, V, kAct><<<grid, kBlock, 0, stream>>>(a, channel_sums);
+    return hipGetLastError();
+}
+
+template <typename T, typename P, int V>
+hipError_t run_activation(const NormArgs& a, bool backward, hipStream_t stream) {
+    switch (a.activation) {
+        case kRelu: return backward ? run_backward<T, P, V, kRelu>(a, stream) : run_forward<T, P, V, kRelu>(a, stream);
+        case kSilu: return backward ? run_backward<T, P, V, kSilu>(a, stream) : run_forward<T, P, V, kSilu>(a, stream);
+        case kGelu: return backward ? run_backward<T, P, V, kGelu>(a, stream) : run_forward<T, P, V, kGelu>(a, stream);
+        default: return backward ? run_backward<T, P, V, kNone>(a, stream) : run_forward<T, P, V, kNone>(a, stream);
+    }
+}
+
+// Vectors of 16 bytes where rows are whole numbers of them and every pointer is
+// aligned to one, else single channels.
+template <typename T, typename P>
+hipError_t run_vectors(const NormArgs& a, bool backward, hipStream_t stream) {
+    constexpr int V = 16 / sizeof(T);
+    const uintptr_t all = reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.y) |
+                          reinterpret_cast<uintptr_t>(a.grad) | reinterpret_cast<uintptr_t>(a.dx);
+    if (a.channels % V == 0 && all % 16 == 0) return run_activation<T, P, V>(a, backward, stream);
+    return run_activation<T, P, 1>(a, backward, stream);
+}
+
+hipError_t run(const NormArgs& a, bool bf16, bool wide_weights, bool backward, hipStream_t stream) {
+    if (!bf16) return run_vectors<float, float>(a, backward, stream);
+    if (wide_weights) return run_vectors<__bf16, float>(a, backward, stream);
+    return run_vectors<__bf16, __bf16>(a, backward, stream);
+}
+
+}  // namespace
+
+int norm_parts(int64_t rows, int clouds, int channels) {
+    // Slices of about 64 KB, and no more work-groups than fill the chip eight
+    // times over.
+    const int64_t mean = (rows + clouds - 1) / clouds;
+    const int64_t by_size = (mean * channels + 16383) / 16384;
+    const int64_t by_fill = std::max<int64_t>(1, 2048 / clouds);
+    return static_cast<int>(std::max<int64_t>(1, std::min(by_size, by_fill)));
+}
+
+int64_t norm_scratch(int64_t rows, int clouds, int channels, int) {
+    return (static_cast<int64_t>(norm_parts(rows, clouds, channels)) + 1) * clouds * channels * 2;
+}
+
+hipError_t launch_norm(const NormArgs& a, bool bf16, bool wide_weights, hipStream_t stream) {
+    return run(a, bf16, wide_weights, false, stream);
+}
+hipError_t launch_norm_backward(const NormArgs& a, bool bf16, bool wide_weights, hipStream_t stream) {
+    return run(a, bf16, wide_weights, true, stream);
+}
+
+}  // namespace tbvh
