@@ -559,8 +559,8 @@ int tbvh_select_blocks(const float* queries, int64_t q_rows, const int64_t* q_st
 /* Attention of every query row over the rows of the key blocks chosen for its
  * block, softmax(scale q.k + bias) v, in bf16 (bf16 = 1) or fp32; a row that is
  * given no keys is zero.  Query head h reads key head h / (heads / kv_heads).
- * Strides are in elements, multiples of 16 bytes, and channels are contiguous; D
- * is a multiple of 8 up to 128.  out, and the backward's gradients, are
+ * Strides are in elements, multiples of 16 bytes, a row's from D to 2^21, and
+ * channels are contiguous; D is a multiple of 8 up to 128.  out, and the backward's gradients, are
  * contiguous.  `selected` entries outside [0, blocks) choose nothing.
  *
  * Bias (table not null): sum over axes a of table[a, map[clamp(q_cells[i, a] -

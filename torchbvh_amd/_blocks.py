@@ -29,6 +29,7 @@ __all__ = ["BlockLayout", "RelativeBias", "block_layout", "block_boxes", "block_
 MAX_BLOCK = 128      # rows of a block
 MAX_SELECTED = 64    # blocks that select_blocks chooses
 MAX_CHANNELS = 128   # channels of a head
+MAX_ROW_STRIDE = 1 << 21  # elements between rows that are read in place
 _TYPES = (torch.float32, torch.bfloat16)
 
 
@@ -49,7 +50,8 @@ class RelativeBias(NamedTuple):
     """A learned bias of the relative position: the sum over axes a of
     ``table[a, buckets[clamp(query_cells[i, a] - key_cells[j, a], -R, R) + R], h]``
     with ``R = len(buckets) // 2``.  Cells are whole numbers, such as
-    coordinates divided by a cell width, or positions in a sequence (one axis)."""
+    coordinates divided by a cell width, or positions in a sequence (one axis);
+    those past 2^28 - 1 either way are taken as that."""
 
     table: torch.Tensor        # (axes, buckets, heads), of the queries' type
     buckets: torch.Tensor      # (2 R + 1,) int32, see `relative_buckets`
@@ -179,7 +181,9 @@ def _rows_of(t: torch.Tensor) -> torch.Tensor:
     start on 16 bytes: the tensor itself where it is so, as slices of one
     projection of queries, keys and values are, else a copy."""
     step = 16 // t.element_size()
-    ok = t.stride(2) == 1 and all(s % step == 0 for s in t.stride()[:2]) and t.data_ptr() % 16 == 0
+    row, head, channel = t.stride()
+    ok = (channel == 1 and row % step == 0 and head % step == 0 and t.data_ptr() % 16 == 0
+          and (t.size(2) <= row <= MAX_ROW_STRIDE or t.size(0) <= 1))
     return t if ok else t.clone(memory_format=torch.contiguous_format)
 
 

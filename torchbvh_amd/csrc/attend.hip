@@ -5,19 +5,39 @@
 namespace tbvh {
 namespace {
 
-constexpr int kChunk = 64;  // keys per step of the running softmax
+constexpr int kChunk = 32;  // keys per step of the running softmax
+
+// The running maximum follows the scores only when one exceeds it by this many
+// powers of two: weights then reach 2^8, which costs their type no precision, and
+// most steps need neither the maximum across lanes nor new sums.
+constexpr float kSlack = 8.0f;
+
+// Waves per SIMD that the registers are kept to (without spills).
+template <typename T>
+constexpr int forward_waves(int DP, int RT, int W, bool bias) {
+    const int words = DP * RT * static_cast<int>(sizeof(T));
+    const int most = words <= 64 ? 4 : words <= 128 ? (sizeof(T) == 4 ? 4 : 3) : words <= 256 ? 3 : words <= 512 ? 2 : 1;
+    const bool tight = words > 128 && (bias || W > 1 || DP == 128);
+    return most - (tight && most > 1 ? 1 : 0);
+}
 
 // One work-group of W waves per (row block, key head, tile of RT * 16 rows of
 // the block's queries times the heads that share the key head); wave w takes
 // every W-th chosen block, and the waves' parts are joined at the end.
 // DP: channels padded to a multiple of 32.
+//
+// A wave holds its queries and sums in registers, takes 32 keys a step straight
+// into the first product's fragments, and turns the values' rows through LDS.
+// The next step's keys and values are loaded while this one's are used.
 template <typename T, int DP, int RT, int W, bool kBias>
-__global__ __launch_bounds__(kWave* W) void attend_kernel(AttendArgs a, int tiles, int64_t items) {
-    constexpr int DS = DP / 32, DT = DP / 16, KT = kChunk / 16;
-    constexpr int LDV = DP + 16 / sizeof(T);  // LDS row stride
+__global__ __launch_bounds__(kWave* W) __attribute__((amdgpu_waves_per_eu(forward_waves<T>(DP, RT, W, kBias)))) void attend_kernel(AttendArgs a, int tiles, int64_t items) {
+    constexpr int DS = DP / 32, DT = DP / 16, KT = kChunk / 16, E = sizeof(T);
+    constexpr int LDV = turned_stride<T>(DP);
+    constexpr int VL = kChunk * DP / 8 / kWave;  // 8-value pieces of a lane
+    constexpr bool kSumByProduct = E == 2;       // fp32 products cost eight times as much
     extern __shared__ float4 s_raw[];
     const int lane = lane_id(), n = lane & 15, g = lane >> 4;
-    const int wave = W == 1 ? 0 : threadIdx.x / kWave;
+    const int wave = W == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int64_t item = xcd_item(blockIdx.x, gridDim.x);
     if (item >= items) return;
     const int c = static_cast<int>(item % a.kv_heads);
@@ -29,8 +49,9 @@ __global__ __launch_bounds__(kWave* W) void attend_kernel(AttendArgs a, int tile
     if (tile * RT * 16 >= rows) return;
 
     T* s_v = reinterpret_cast<T*>(s_raw) + wave * kChunk * LDV;
-    float* s_bias = reinterpret_cast<float*>(reinterpret_cast<T*>(s_raw) + W * kChunk * LDV);
-    const int span = 2 * a.reach + 1, entries = a.axes * span;
+    int* s_cell = reinterpret_cast<int*>(reinterpret_cast<T*>(s_raw) + W * kChunk * LDV) + wave * 3 * kChunk;
+    float* s_bias = reinterpret_cast<float*>(reinterpret_cast<T*>(s_raw) + W * kChunk * LDV) + W * 3 * kChunk;
+    const int span = 2 * a.reach + 1, entries = a.axes * span, reach = 4 * a.reach;
     if constexpr (kBias) {
         const T* table = static_cast<const T*>(a.table);
         for (int i = threadIdx.x; i < a.share * entries; i += kWave * W) {
@@ -41,9 +62,12 @@ __global__ __launch_bounds__(kWave* W) void attend_kernel(AttendArgs a, int tile
         __syncthreads();
     }
 
+    // Scores in powers of two are fma(s, to_log2, bias); a negative scale goes into
+    // the queries, so the largest score is the largest product.
+    const float to_log2 = fabsf(a.scale) * kLog2e;
     Vec8<T> qf[RT][DS];
     int qc[RT][3];
-    const float* bias_row[RT];
+    const char* bias_row[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         const int rr = tile * RT * 16 + rt * 16 + n;
@@ -51,121 +75,212 @@ __global__ __launch_bounds__(kWave* W) void attend_kernel(AttendArgs a, int tile
         const int qi = real ? rr / a.share : 0, hs = real ? rr - qi * a.share : 0;
         const T* row = static_cast<const T*>(a.q) + (qr.first + qi) * a.q_row + (c * a.share + hs) * a.q_head;
 #pragma unroll
-        for (int s = 0; s < DS; ++s) qf[rt][s] = load8(row, 32 * s + 8 * g, a.D, real);
+        for (int s = 0; s < DS; ++s) {
+            qf[rt][s] = load8(row, 32 * s + 8 * g, a.D, real);
+            if (a.scale < 0.0f) qf[rt][s] = -qf[rt][s];
+        }
         if constexpr (kBias) {
-            bias_row[rt] = s_bias + hs * entries;
+            bias_row[rt] = reinterpret_cast<const char*>(s_bias + hs * entries + a.reach);
 #pragma unroll
-            for (int x = 0; x < 3; ++x) qc[rt][x] = x < a.axes ? a.q_cells[(qr.first + qi) * a.axes + x] : 0;
+            for (int x = 0; x < 3; ++x) qc[rt][x] = x < a.axes ? cell_bytes(a.q_cells[(qr.first + qi) * a.axes + x]) : 0;
         }
     }
 
-    f32x4 acc[RT][DT];
+    f32x4 acc[RT][DT], sums[RT];
     float top[RT], sum[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         top[rt] = -INFINITY;
         sum[rt] = 0.0f;
+        sums[rt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int t = 0; t < DT; ++t) acc[rt][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    const float to_log2 = a.scale * kLog2e;
+    // A score in units of `unit` powers of two: with a bias they are converted first.
+    const float unit = kBias ? 1.0f : to_log2;
+    const float slack = unit > 0.0f ? kSlack / unit : 3.0e38f;
+    Vec8<T> ones;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) ones[j] = static_cast<T>(1.0f);
 
-    for (int slot = wave; slot < a.count; slot += W) {
-        const int block = __builtin_amdgcn_readfirstlane(a.selected[group * a.count + slot]);
-        if (block < 0 || block >= a.blocks) continue;
-        const Rows kr = block_rows(a.k_starts, block, a.k_block, a.k_total);
-        for (int base = 0; base < kr.count; base += kChunk) {
-            const T* k0 = static_cast<const T*>(a.k) + (kr.first + base) * a.k_row + c * a.k_head;
-            const T* v0 = static_cast<const T*>(a.v) + (kr.first + base) * a.v_row + c * a.v_head;
+    // A lane's byte offsets into a step's keys and values.
+    uint32_t k_at[KT][DS], v_at[VL];
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int s = 0; s < DS; ++s) {
+            const int d = 32 * s + 8 * g;
+            k_at[kt][s] = d < a.D ? static_cast<uint32_t>((16 * kt + n) * a.k_row + d) * E : kNowhere;
+        }
+#pragma unroll
+    for (int i = 0; i < VL; ++i) {
+        const int p = lane + kWave * i, d = p % (DP / 8) * 8;
+        v_at[i] = d < a.D ? static_cast<uint32_t>(p / (DP / 8) * a.v_row + d) * E : kNowhere;
+    }
+
+    for (int from = 0; from < a.count; from += kWave) {
+        const int slots = min(a.count - from, kWave);
+        Slots list;
+        list.load(a.selected + group * a.count + from, slots, a.blocks, a.k_starts, a.k_block, a.k_total);
+        int slot = wave, base = 0;
+        Rows kr = {0, 0};
+        const auto skip = [&] {  // to the next chosen block that has rows
+            kr.count = 0;
+            while (slot < slots && (kr = list.at(slot)).count == 0) slot += W;
+        };
+        Vec8<T> kf[KT][DS], vs[VL];
+        int cells[3];
+        const auto load_keys = [&] {
+            const Buffer kb = rows_buffer<T>(a.k, kr.first + base, c * a.k_head, kr.count - base, a.k_row, a.D);
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                for (int s = 0; s < DS; ++s) kf[kt][s] = load8<T>(kb, k_at[kt][s]);
+        };
+        const auto load_values = [&] {
+            const Buffer vb = rows_buffer<T>(a.v, kr.first + base, c * a.v_head, kr.count - base, a.v_row, a.D);
+#pragma unroll
+            for (int i = 0; i < VL; ++i) vs[i] = load8<T>(vb, v_at[i]);
+            if constexpr (kBias) {
+                const int64_t row = kr.first + base + min(lane & (kChunk - 1), max(kr.count - base - 1, 0));
+#pragma unroll
+                for (int x = 0; x < 3; ++x)
+                    if (x < a.axes) cells[x] = a.k_cells[row * a.axes + x];
+            }
+        };
+        skip();
+        if (slot < slots) {
+            load_values();
+            load_keys();
+        }
+        while (slot < slots) {
             const int left = kr.count - base;
             wave_sync();
 #pragma unroll
-            for (int i = 0; i < DP / 8; ++i) {
-                const int p = lane + kWave * i, row = p / (DP / 8), d = p % (DP / 8) * 8;
-                *reinterpret_cast<Vec8<T>*>(s_v + row * LDV + d) = load8(v0 + row * a.v_row, d, a.D, row < left);
+            for (int i = 0; i < VL; ++i) {
+                const int p = lane + kWave * i;
+                *reinterpret_cast<Vec8<T>*>(s_v + p / (DP / 8) * LDV + p % (DP / 8) * 8) = vs[i];
             }
+            if constexpr (kBias) {
+#pragma unroll
+                for (int x = 0; x < 3; ++x)
+                    if (x < a.axes) s_cell[x * kChunk + (lane & (kChunk - 1))] = cell_bytes(cells[x]);
+            }
+            wave_sync();
+            base += kChunk;
+            if (base >= kr.count) {
+                base = 0;
+                slot += W;
+                skip();
+            }
+            if (slot < slots) load_values();
             f32x4 st[KT][RT];
 #pragma unroll
-            for (int kt = 0; kt < KT; ++kt) {
-                Vec8<T> kf[DS];
-                const int row = 16 * kt + n;
-#pragma unroll
-                for (int s = 0; s < DS; ++s) kf[s] = load8(k0 + row * a.k_row, 32 * s + 8 * g, a.D, row < left);
+            for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) {
-                    f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+                    st[kt][rt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                    for (int s = 0; s < DS; ++s) x = mma(kf[s], qf[rt][s], x);
-                    st[kt][rt] = x * to_log2;
+                    for (int s = 0; s < DS; ++s) st[kt][rt] = mma(kf[kt][s], qf[rt][s], st[kt][rt]);
                 }
-                if constexpr (kBias) {
-                    for (int x = 0; x < a.axes; ++x) {
+            if (slot < slots) load_keys();
+            if constexpr (kBias) {
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const int key = min(16 * kt + 4 * g + r, left - 1);
-                            const int kc = a.k_cells[(kr.first + base + key) * a.axes + x];
+                for (int kt = 0; kt < KT; ++kt) {
 #pragma unroll
-                            for (int rt = 0; rt < RT; ++rt) {
-                                const int q = x == 0 ? qc[rt][0] : x == 1 ? qc[rt][1] : qc[rt][2];
-                                st[kt][rt][r] += bias_row[rt][x * span + cell_offset(q, kc, a.reach)];
-                            }
-                        }
+                    for (int rt = 0; rt < RT; ++rt) st[kt][rt] *= to_log2;
+#pragma unroll
+                    for (int x = 0; x < 3; ++x) {
+                        if (x >= a.axes) continue;
+                        const int4 kc = *reinterpret_cast<const int4*>(s_cell + x * kChunk + 16 * kt + 4 * g);
+                        const int key[4] = {kc.x, kc.y, kc.z, kc.w};
+#pragma unroll
+                        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r)
+                                st[kt][rt][r] += *reinterpret_cast<const float*>(
+                                    bias_row[rt] + x * span * 4 + cell_distance(qc[rt][x], key[r], reach));
                     }
                 }
-                if (left < kChunk) {
+            }
+            if (left < kChunk) {
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
                         if (16 * kt + 4 * g + r >= left)
 #pragma unroll
                             for (int rt = 0; rt < RT; ++rt) st[kt][rt][r] = -INFINITY;
-                }
             }
-            Vec8<T> pf[KT / 2][RT];
+            float most[RT];
+            bool above = false;
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
-                float m = -INFINITY;
+                float m = fmaxf(fmaxf(st[0][rt][0], st[0][rt][1]), fmaxf(st[0][rt][2], st[0][rt][3]));
 #pragma unroll
-                for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) m = fmaxf(m, st[kt][rt][r]);
-                m = fmaxf(top[rt], across_groups_max(m));
-                // Rows that have met no finite score yet keep weights of zero.
-                const float ref = m == -INFINITY ? 0.0f : m;
-                const float keep = __builtin_amdgcn_exp2f(top[rt] - ref);
-                top[rt] = m;
-                float part = 0.0f;
-#pragma unroll
-                for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        st[kt][rt][r] = __builtin_amdgcn_exp2f(st[kt][rt][r] - ref);
-                        part += st[kt][rt][r];
-                    }
-                sum[rt] = sum[rt] * keep + part;
-#pragma unroll
-                for (int t = 0; t < DT; ++t) acc[rt][t] *= keep;
-                // Weights are rounded to T for the product with v (2^-9 each in
-                // bf16, independent); their sum is kept in fp32.
-#pragma unroll
-                for (int p = 0; p < KT / 2; ++p) pf[p][rt] = join<T>(st[2 * p][rt], st[2 * p + 1][rt]);
+                for (int kt = 1; kt < KT; ++kt)
+                    m = fmaxf(fmaxf(fmaxf(m, st[kt][rt][0]), fmaxf(st[kt][rt][1], st[kt][rt][2])), st[kt][rt][3]);
+                most[rt] = m;
+                above |= m > top[rt] + slack;
             }
-            wave_sync();
+            if (__any(above)) {
 #pragma unroll
-            for (int p = 0; p < KT / 2; ++p)
+                for (int rt = 0; rt < RT; ++rt) {
+                    const float m = fmaxf(top[rt], across_groups_max(most[rt]));
+                    const float keep = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((top[rt] - m) * unit);
+                    top[rt] = m;
+                    sum[rt] *= keep;
+                    sums[rt] *= keep;
 #pragma unroll
-                for (int t = 0; t < DT; ++t) {
-                    Vec8<T> vf;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        vf[j] = s_v[(32 * p + 16 * (j / 4) + 4 * g + j % 4) * LDV + 16 * t + n];
-#pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) acc[rt][t] = mma(vf, pf[p][rt], acc[rt][t]);
+                    for (int t = 0; t < DT; ++t) acc[rt][t] *= keep;
                 }
+            }
+            // Weights are rounded to T for the product with v (2^-9 each in bf16,
+            // independent); the sums are of the same rounded weights, in fp32.
+            Vec8<T> pf[RT];
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                // Rows that have met no finite score yet keep weights of zero.
+                const float ref = top[rt] == -INFINITY ? 0.0f : -top[rt] * unit;
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        st[kt][rt][r] = __builtin_amdgcn_exp2f(kBias ? st[kt][rt][r] + ref
+                                                                     : __builtin_fmaf(st[kt][rt][r], unit, ref));
+            }
+            if (left < kChunk) {
+                // Not left to exp2(-inf): a scale of zero would make it undefined.
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (16 * kt + 4 * g + r >= left)
+#pragma unroll
+                            for (int rt = 0; rt < RT; ++rt) st[kt][rt][r] = 0.0f;
+            }
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                pf[rt] = join<T>(st[0][rt], st[1][rt]);
+                if constexpr (kSumByProduct) {
+                    sums[rt] = mma(ones, pf[rt], sums[rt]);
+                } else {
+#pragma unroll
+                    for (int kt = 0; kt < KT; ++kt)
+                        sum[rt] += (st[kt][rt][0] + st[kt][rt][1]) + (st[kt][rt][2] + st[kt][rt][3]);
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < DT; ++t) {
+                const Vec8<T> vf = load_turned<T, LDV>(s_v, t, n, g);
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) acc[rt][t] = mma(vf, pf[rt], acc[rt][t]);
+            }
         }
     }
 
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) sum[rt] = across_groups_sum(sum[rt]);
+    for (int rt = 0; rt < RT; ++rt) sum[rt] = kSumByProduct ? sums[rt][0] : across_groups_sum(sum[rt]);
     if constexpr (W > 1) {
         // Every wave's (top, sum, acc) through LDS; wave 0 joins them in order.
         float* s_part = reinterpret_cast<float*>(s_raw);
@@ -188,13 +303,15 @@ __global__ __launch_bounds__(kWave* W) void attend_kernel(AttendArgs a, int tile
             const float* p = s_part + rt * (DT * 4 + 2) * kWave + lane;
             float m = top[rt];
             for (int w = 1; w < W; ++w) m = fmaxf(m, p[w * kPer]);
-            const float ref = m == -INFINITY ? 0.0f : m;
-            const float keep = __builtin_amdgcn_exp2f(top[rt] - ref);
+            const auto weight = [&](float t) {
+                return t == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((t - m) * unit);
+            };
+            const float keep = weight(top[rt]);
             sum[rt] *= keep;
 #pragma unroll
             for (int t = 0; t < DT; ++t) acc[rt][t] *= keep;
             for (int w = 1; w < W; ++w) {
-                const float f = __builtin_amdgcn_exp2f(p[w * kPer] - ref);
+                const float f = weight(p[w * kPer]);
                 sum[rt] += p[w * kPer + kWave] * f;
 #pragma unroll
                 for (int t = 0; t < DT; ++t)
@@ -224,7 +341,8 @@ __global__ __launch_bounds__(kWave* W) void attend_kernel(AttendArgs a, int tile
             }
         }
         // 0 for an empty row: its scores are all -inf, their weights 0 again.
-        if (a.lse != nullptr && g == 0) a.lse[at] = sum[rt] == 0.0f ? 0.0f : top[rt] + __builtin_amdgcn_logf(sum[rt]);
+        if (a.lse != nullptr && g == 0)
+            a.lse[at] = sum[rt] == 0.0f ? 0.0f : __builtin_fmaf(top[rt], unit, __builtin_amdgcn_logf(sum[rt]));
     }
 }
 
@@ -233,8 +351,9 @@ hipError_t launch(const AttendArgs& a, hipStream_t stream) {
     const int tiles = (a.q_block * a.share + RT * 16 - 1) / (RT * 16);
     const int64_t items = static_cast<int64_t>(a.groups) * tiles * a.kv_heads;
     const unsigned grid = static_cast<unsigned>(xcd_grid(items));
-    const size_t stage = static_cast<size_t>(W) * kChunk * (DP + 16 / sizeof(T)) * sizeof(T);
-    const size_t bias = static_cast<size_t>(a.share) * a.axes * (2 * a.reach + 1) * sizeof(float);
+    const size_t stage = static_cast<size_t>(W) * kChunk * turned_stride<T>(DP) * sizeof(T);
+    const size_t bias = static_cast<size_t>(W) * 3 * kChunk * sizeof(int) +
+                        static_cast<size_t>(a.share) * a.axes * (2 * a.reach + 1) * sizeof(float);
     const size_t parts = W > 1 ? static_cast<size_t>(W) * RT * (DP / 16 * 4 + 2) * kWave * sizeof(float) : 0;
     if (a.table != nullptr) {
         const auto kernel = attend_kernel<T, DP, RT, W, true>;
@@ -264,8 +383,7 @@ hipError_t launch_rows(const AttendArgs& a, hipStream_t stream) {
     constexpr int64_t kFill = 2048;  // waves that fill the 256 CUs twice a SIMD
     if (rows <= 16) {
         const int64_t items = static_cast<int64_t>(a.groups) * a.kv_heads;
-        // Eight waves' staged values fit the LDS but for fp32 rows of 128.
-        constexpr int kMany = sizeof(T) * DP <= 256 ? 8 : 4;
+        constexpr int kMany = DP <= 64 ? 8 : 4;
         if (items * 4 <= kFill && a.count > 1) return launch<T, DP, 1, kMany>(a, stream);
         return launch<T, DP, 1, 1>(a, stream);
     }

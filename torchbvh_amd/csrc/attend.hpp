@@ -56,6 +56,37 @@ __device__ __forceinline__ f32x4 mma(f32x8 a, f32x8 b, f32x4 c) {
     return c;
 }
 
+// Rows of a block as a buffer: a load past `bytes` gives zeros and touches no
+// memory, so neither the rows after a short block nor the channels after D
+// need a branch.
+using Buffer = __amdgpu_buffer_rsrc_t;
+constexpr uint32_t kNowhere = 0x7fff0000u;
+__device__ __forceinline__ Buffer buffer(const void* first, int64_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(first), 0, static_cast<int>(max(bytes, int64_t{0})),
+                                             0x00027000);
+}
+using Words4 = uint32_t __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ Words4 load16(Buffer b, uint32_t at) {
+    return __builtin_bit_cast(Words4, __builtin_amdgcn_raw_buffer_load_b128(b, at, 0, 0));
+}
+// Eight values from byte `at` on.
+template <typename T>
+__device__ __forceinline__ Vec8<T> load8(Buffer b, uint32_t at) {
+    if constexpr (sizeof(T) == 2) {
+        return __builtin_bit_cast(Vec8<T>, load16(b, at));
+    } else {
+        const f32x4 x = __builtin_bit_cast(f32x4, load16(b, at)), y = __builtin_bit_cast(f32x4, load16(b, at + 16));
+        return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+}
+// Rows `count` of `stride` elements, D of each in use.
+template <typename T>
+__device__ __forceinline__ Buffer rows_buffer(const void* base, int64_t first, int64_t offset, int count, int64_t stride,
+                                              int D) {
+    return buffer(static_cast<const T*>(base) + first * stride + offset,
+                  count > 0 ? ((count - 1) * stride + D) * static_cast<int64_t>(sizeof(T)) : 0);
+}
+
 // Eight channels from channel d of a row; zeros past D (a multiple of 8).
 template <typename T>
 __device__ __forceinline__ Vec8<T> load8(const T* __restrict__ row, int d, int D, bool real) {
@@ -63,6 +94,30 @@ __device__ __forceinline__ Vec8<T> load8(const T* __restrict__ row, int d, int D
     if (real && d < D) v = *reinterpret_cast<const Vec8<T>*>(row + d);
     return v;
 }
+
+// The operand that is contracted along rows 0..31 of an LDS tile (row stride
+// LD), for columns 16 t + n: rows 4 g + j of each half.  Two transposed reads in
+// bf16: in a group of 16 lanes, lane l's 8 bytes are row l / 4's columns
+// 4 (l % 4) .. + 3, and the read hands lane n column n of the four rows.
+template <typename T, int LD>
+__device__ __forceinline__ Vec8<T> load_turned(const T* tile, int t, int n, int g) {
+    if constexpr (sizeof(T) == 2) {
+        using Lds = __attribute__((address_space(3))) bf16x4;
+        const T* at = tile + (4 * g + n / 4) * LD + 16 * t + 4 * (n % 4);
+        const bf16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((Lds*)at);
+        const bf16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((Lds*)(at + 16 * LD));
+        return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    } else {
+        Vec8<T> v;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = tile[(16 * (j / 4) + 4 * g + j % 4) * LD + 16 * t + n];
+        return v;
+    }
+}
+// Row stride of such a tile: in bf16 eight rows' 32-byte pieces then fall on
+// 64 different banks.
+template <typename T>
+constexpr int turned_stride(int DP) { return sizeof(T) == 2 ? DP + 16 : DP + 4; }
 
 template <typename T>
 __device__ __forceinline__ Vec8<T> join(f32x4 a, f32x4 b) {
@@ -156,11 +211,33 @@ __device__ __forceinline__ float across_groups_sum(float v) {
     return v + __shfl_xor(v, 32, kWave);
 }
 
-// Distance of two cells on an axis, clamped to [-reach, reach], from zero up.
-__device__ __forceinline__ int cell_offset(int a, int b, int reach) {
-    const int d = __builtin_elementwise_sub_sat(a, b);
-    return min(max(d, -reach), reach) + reach;
-}
+// Cells are held as byte offsets into a table of floats, and far ones at the ends
+// of a range whose differences cannot overflow.
+constexpr int kFarCell = (1 << 28) - 1;
+__device__ __forceinline__ int cell_bytes(int cell) { return min(max(cell, -kFarCell), kFarCell) * 4; }
+// The distance of two such cells, clamped to [-reach, reach] (in bytes).
+__device__ __forceinline__ int cell_distance(int a, int b, int reach) { return min(max(a - b, -reach), reach); }
+
+// The key blocks chosen for a row block, 64 slots at a time: lane i holds slot
+// i's rows, and walking them needs no further loads.
+struct Slots {
+    int first_lo, first_hi, count;
+    __device__ __forceinline__ void load(const int32_t* __restrict__ selected, int slots, int blocks,
+                                         const int64_t* __restrict__ starts, int block, int64_t total) {
+        const int lane = lane_id();
+        const int b = lane < slots ? selected[lane] : -1;
+        Rows r = {0, 0};
+        if (b >= 0 && b < blocks) r = block_rows(starts, b, block, total);
+        first_lo = static_cast<int>(r.first);
+        first_hi = static_cast<int>(r.first >> 32);
+        count = r.count;
+    }
+    __device__ __forceinline__ Rows at(int slot) const {
+        const uint32_t lo = __builtin_amdgcn_readlane(first_lo, slot);
+        const int64_t hi = __builtin_amdgcn_readlane(first_hi, slot);
+        return {hi << 32 | lo, __builtin_amdgcn_readlane(count, slot)};
+    }
+};
 
 hipError_t launch_attend(const AttendArgs& a, bool bf16, hipStream_t stream);
 hipError_t launch_attend_backward(const AttendArgs& a, const AttendGrads& g, bool bf16, hipStream_t stream);

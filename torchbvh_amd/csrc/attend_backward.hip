@@ -82,7 +82,7 @@ __global__ __launch_bounds__(kWave) void attend_dq_kernel(AttendArgs a, AttendGr
             if (real && g == 0) gr.delta[row * a.heads + h] = delta[rt];
             if constexpr (kBias) {
 #pragma unroll
-                for (int x = 0; x < 3; ++x) qc[rt][x] = x < a.axes ? a.q_cells[row * a.axes + x] : 0;
+                for (int x = 0; x < 3; ++x) qc[rt][x] = x < a.axes ? cell_bytes(a.q_cells[row * a.axes + x]) : 0;
             }
         }
         f32x4 acc[RT][DT];
@@ -124,11 +124,11 @@ __global__ __launch_bounds__(kWave) void attend_dq_kernel(AttendArgs a, AttendGr
 #pragma unroll
                             for (int r = 0; r < 4; ++r) {
                                 const int key = min(16 * kt + 4 * g + r, left - 1);
-                                const int kc = a.k_cells[(kr.first + base + key) * a.axes + x];
+                                const int kc = cell_bytes(a.k_cells[(kr.first + base + key) * a.axes + x]);
 #pragma unroll
                                 for (int rt = 0; rt < RT; ++rt) {
                                     const int q = x == 0 ? qc[rt][0] : x == 1 ? qc[rt][1] : qc[rt][2];
-                                    st[rt][r] += s_bias[x * span + cell_offset(q, kc, a.reach)];
+                                    st[rt][r] += s_bias[x * span + a.reach + cell_distance(q, kc, 4 * a.reach) / 4];
                                 }
                             }
                         }
@@ -151,11 +151,11 @@ __global__ __launch_bounds__(kWave) void attend_dq_kernel(AttendArgs a, AttendGr
 #pragma unroll
                             for (int r = 0; r < 4; ++r) {
                                 const int key = min(16 * kt + 4 * g + r, left - 1);
-                                const int kc = a.k_cells[(kr.first + base + key) * a.axes + x];
+                                const int kc = cell_bytes(a.k_cells[(kr.first + base + key) * a.axes + x]);
 #pragma unroll
                                 for (int rt = 0; rt < RT; ++rt) {
                                     const int q = x == 0 ? qc[rt][0] : x == 1 ? qc[rt][1] : qc[rt][2];
-                                    float* bin = s_sum + s_bin[x * span + cell_offset(q, kc, a.reach)] + lane;
+                                    float* bin = s_sum + s_bin[x * span + a.reach + cell_distance(q, kc, 4 * a.reach) / 4] + lane;
                                     *bin += ds[kt][rt][r];
                                 }
                             }
@@ -266,7 +266,7 @@ __global__ __launch_bounds__(kWave) void attend_dkv_kernel(AttendArgs a, AttendG
         }
         if constexpr (kBias) {
 #pragma unroll
-            for (int x = 0; x < 3; ++x) kc[kt][x] = x < a.axes ? a.k_cells[at * a.axes + x] : 0;
+            for (int x = 0; x < 3; ++x) kc[kt][x] = x < a.axes ? cell_bytes(a.k_cells[at * a.axes + x]) : 0;
         }
     }
     f32x4 dk[KT][DT], dv[KT][DT];
@@ -313,7 +313,7 @@ __global__ __launch_bounds__(kWave) void attend_dkv_kernel(AttendArgs a, AttendG
                 if constexpr (kBias) {
                     s_head[16 * rt + n] = hs * entries;
                     for (int x = 0; x < a.axes; ++x)
-                        s_cell[x * kStep + 16 * rt + n] = real ? a.q_cells[row * a.axes + x] : 0;
+                        s_cell[x * kStep + 16 * rt + n] = real ? cell_bytes(a.q_cells[row * a.axes + x]) : 0;
                 }
             }
         }
@@ -338,7 +338,7 @@ __global__ __launch_bounds__(kWave) void attend_dkv_kernel(AttendArgs a, AttendG
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
                             const int q = 16 * rt + 4 * g + r;
-                            x[r] += s_bias[s_head[q] + ax * span + cell_offset(s_cell[ax * kStep + q], key, a.reach)];
+                            x[r] += s_bias[s_head[q] + ax * span + a.reach + cell_distance(s_cell[ax * kStep + q], key, 4 * a.reach) / 4];
                         }
                     }
                 }

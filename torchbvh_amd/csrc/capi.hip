@@ -1546,6 +1546,8 @@ int tbvh_interpolate_backward(const float* grad, const int64_t* indices, const f
 namespace {
 constexpr int64_t kMaxGroups = int64_t{1} << 26;  // work-groups of 64 lanes that one launch holds
 
+constexpr int64_t kMaxRowStride = int64_t{1} << 21;
+
 bool multiple_of_16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 // Forward and backward alike: the kernels' arguments, after every size, stride
@@ -1579,6 +1581,12 @@ int check_attend(const char* op, const tbvh_attend_args* x, AttendArgs& a) {
     if (strides * (x->bf16 ? 2 : 4) % 16 != 0 || !multiple_of_16(x->q) || !multiple_of_16(x->k) || !multiple_of_16(x->v) ||
         !multiple_of_16(x->out)) {
         return fail(TBVH_ERR_INVALID_ARGUMENT, "%s: q, k, v and out must be 16-byte aligned, and their strides", op);
+    }
+    // A block's rows are addressed with 31 bits.
+    for (const int64_t stride : {x->q_row_stride, x->k_row_stride, x->v_row_stride}) {
+        if (stride < 0 || stride > kMaxRowStride) {
+            return fail(TBVH_ERR_INVALID_ARGUMENT, "%s: row strides must be 0 to 2^21 elements", op);
+        }
     }
     if (x->table) {
         if (x->axes < 1 || x->axes > 3 || x->buckets < 1 || x->reach < 0 || x->axes * int64_t{x->buckets} > kMaxBins ||
