@@ -51,7 +51,7 @@ class RelativeBias(NamedTuple):
     ``table[a, buckets[clamp(query_cells[i, a] - key_cells[j, a], -R, R) + R], h]``
     with ``R = len(buckets) // 2``.  Cells are whole numbers, such as
     coordinates divided by a cell width, or positions in a sequence (one axis);
-    those past 2^28 - 1 either way are taken as that."""
+    those past 2^26 either way are taken as that."""
 
     table: torch.Tensor        # (axes, buckets, heads), of the queries' type
     buckets: torch.Tensor      # (2 R + 1,) int32, see `relative_buckets`
@@ -193,10 +193,10 @@ class _Attend(torch.autograd.Function):
         q, k, v = _rows_of(q), _rows_of(k), _rows_of(v)
         bias = None if table is None else (table, *places)
         wanted = any(ctx.needs_input_grad[:4])
-        out, lse = _C.attend(q, k, v, selected, query_layout.starts, key_layout.starts, query_layout.block_size,
-                             key_layout.block_size, scale, bias, wanted)
+        out, lse, rest = _C.attend(q, k, v, selected, query_layout.starts, key_layout.starts, query_layout.block_size,
+                                   key_layout.block_size, scale, bias, wanted)
         if wanted:
-            ctx.save_for_backward(q, k, v, out, lse, table, selected, query_layout.starts, key_layout.starts,
+            ctx.save_for_backward(q, k, v, out, lse, rest, table, selected, query_layout.starts, key_layout.starts,
                                   *(places or ()))
             ctx.sizes = (query_layout.block_size, key_layout.block_size, scale)
         return out
@@ -204,12 +204,12 @@ class _Attend(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        q, k, v, out, lse, table, selected, q_starts, k_starts, *places = ctx.saved_tensors
+        q, k, v, out, lse, rest, table, selected, q_starts, k_starts, *places = ctx.saved_tensors
         if 0 in (q.numel(), k.numel(), selected.numel(), k_starts.numel() - 1):
             grads = [torch.zeros_like(t) for t in (q, k, v)] + [None if table is None else torch.zeros_like(table)]
         else:
             bias = None if table is None else (table, *places)
-            grads = _C.attend_backward(_rows_of(grad.contiguous()), q, k, v, out, lse, selected, q_starts, k_starts,
+            grads = _C.attend_backward(_rows_of(grad.contiguous()), q, k, v, out, lse, rest, selected, q_starts, k_starts,
                                        *ctx.sizes, bias)
         return *grads, None, None, None, None, None
 

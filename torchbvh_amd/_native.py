@@ -53,7 +53,7 @@ class AttendArgs(ctypes.Structure):
         + [("scale", ctypes.c_float)]
         + [(n, _vp) for n in ("table", "map", "q_cells", "k_cells")]
         + [(n, ctypes.c_int32) for n in ("axes", "buckets", "reach")]
-        + [(n, _vp) for n in ("out", "lse")]
+        + [(n, _vp) for n in ("out", "lse", "rest")]
     )
 
 
@@ -249,6 +249,10 @@ def _check(status: int) -> None:
 
 def _ptr(t: torch.Tensor | None):
     return None if t is None else ctypes.c_void_p(t.data_ptr())
+
+
+def _address(t: torch.Tensor | None):
+    return None if t is None else t.data_ptr()
 
 
 def _stream(device: torch.device):
@@ -1260,23 +1264,25 @@ class _NativeOps:
     def attend(q, k, v, selected, q_starts, k_starts, q_block, k_block, scale, bias, want_lse):
         """`tbvh_attend`: q (rows, heads, D), k and v (rows, kv_heads, D) with
         contiguous channels; `bias` None or (table, map, q_cells, k_cells).
-        Returns the output and, if wanted, its log-sum-exp in base 2."""
+        Returns the output and, if wanted, its log-sum-exp in base 2 and, in
+        bfloat16 with a bias, what the output's rounding left off."""
         args = _attend_args("attend", q, k, v, selected, q_starts, k_starts, q_block, k_block, scale, bias)
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if want_lse else None
-        args.out, args.lse = out.data_ptr(), None if lse is None else lse.data_ptr()
+        lse = torch.empty((q.size(1), q.size(0)), dtype=torch.float32, device=q.device) if want_lse else None
+        rest = torch.empty_like(out) if want_lse and bias is not None and q.dtype == torch.bfloat16 else None
+        args.out, args.lse, args.rest = out.data_ptr(), lse.data_ptr() if want_lse else None, _address(rest)
         with torch.cuda.device(q.device):
             _check(load().tbvh_attend(ctypes.byref(args), _stream(q.device)))
-        return out, lse
+        return out, lse, rest
 
     @staticmethod
-    def attend_backward(grad, q, k, v, out, lse, selected, q_starts, k_starts, q_block, k_block, scale, bias):
+    def attend_backward(grad, q, k, v, out, lse, rest, selected, q_starts, k_starts, q_block, k_block, scale, bias):
         """`tbvh_attend_backward`: (dq, dk, dv, dtable or None)."""
         op = "attend_backward"
         _require(grad.shape == q.shape and grad.is_contiguous() and grad.dtype == q.dtype, op,
                  "grad must be contiguous, of q's shape and type")
         args = _attend_args(op, q, k, v, selected, q_starts, k_starts, q_block, k_block, scale, bias)
-        args.out, args.lse = out.data_ptr(), lse.data_ptr()
+        args.out, args.lse, args.rest = out.data_ptr(), lse.data_ptr(), _address(rest)
         dev = q.device
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
         dtable = None if bias is None else torch.empty(bias[0].shape, dtype=q.dtype, device=dev)

@@ -99,6 +99,10 @@ __global__ __launch_bounds__(kWave* W) __attribute__((amdgpu_waves_per_eu(forwar
     // A score in units of `unit` powers of two: with a bias they are converted first.
     const float unit = kBias ? 1.0f : to_log2;
     const float slack = unit > 0.0f ? kSlack / unit : 3.0e38f;
+    // A table's gradient is a sum in which each row's scores cancel, down to the
+    // error of delta = grad . out; so where it is wanted the weights take part with
+    // what their rounding left off, too, and so is the output kept.
+    const bool exact = a.rest != nullptr;
     Vec8<T> ones;
 #pragma unroll
     for (int j = 0; j < 8; ++j) ones[j] = static_cast<T>(1.0f);
@@ -237,7 +241,7 @@ __global__ __launch_bounds__(kWave* W) __attribute__((amdgpu_waves_per_eu(forwar
             }
             // Weights are rounded to T for the product with v (2^-9 each in bf16,
             // independent); the sums are of the same rounded weights, in fp32.
-            Vec8<T> pf[RT];
+            Vec8<T> pf[RT], lo[RT];
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
                 // Rows that have met no finite score yet keep weights of zero.
@@ -264,6 +268,12 @@ __global__ __launch_bounds__(kWave* W) __attribute__((amdgpu_waves_per_eu(forwar
                 pf[rt] = join<T>(st[0][rt], st[1][rt]);
                 if constexpr (kSumByProduct) {
                     sums[rt] = mma(ones, pf[rt], sums[rt]);
+                    if (kBias && exact) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            lo[rt][j] = static_cast<T>(st[j / 4][rt][j % 4] - static_cast<float>(pf[rt][j]));
+                        sums[rt] = mma(ones, lo[rt], sums[rt]);
+                    }
                 } else {
 #pragma unroll
                     for (int kt = 0; kt < KT; ++kt)
@@ -274,7 +284,10 @@ __global__ __launch_bounds__(kWave* W) __attribute__((amdgpu_waves_per_eu(forwar
             for (int t = 0; t < DT; ++t) {
                 const Vec8<T> vf = load_turned<T, LDV>(s_v, t, n, g);
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt) acc[rt][t] = mma(vf, pf[rt], acc[rt][t]);
+                for (int rt = 0; rt < RT; ++rt) {
+                    acc[rt][t] = mma(vf, pf[rt], acc[rt][t]);
+                    if (kSumByProduct && kBias && exact) acc[rt][t] = mma(vf, lo[rt], acc[rt][t]);
+                }
             }
         }
     }
@@ -338,11 +351,19 @@ __global__ __launch_bounds__(kWave* W) __attribute__((amdgpu_waves_per_eu(forwar
 #pragma unroll
                 for (int r = 0; r < 4; ++r) o[r] = static_cast<T>(acc[rt][t][r] * inverse);
                 *reinterpret_cast<Vec4<T>*>(row + d) = o;
+                if (kSumByProduct && kBias && exact) {
+                    Vec4<T> left;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        left[r] = static_cast<T>(__builtin_fmaf(acc[rt][t][r], inverse, -static_cast<float>(o[r])));
+                    *reinterpret_cast<Vec4<T>*>(static_cast<T*>(a.rest) + at * a.D + d) = left;
+                }
             }
         }
         // 0 for an empty row: its scores are all -inf, their weights 0 again.
         if (a.lse != nullptr && g == 0)
-            a.lse[at] = sum[rt] == 0.0f ? 0.0f : __builtin_fmaf(top[rt], unit, __builtin_amdgcn_logf(sum[rt]));
+            a.lse[(c * a.share + hs) * a.q_total + qr.first + qi] =
+                sum[rt] == 0.0f ? 0.0f : __builtin_fmaf(top[rt], unit, __builtin_amdgcn_logf(sum[rt]));
     }
 }
 

@@ -130,6 +130,18 @@ __device__ __forceinline__ Vec8<T> join(f32x4 a, f32x4 b) {
     return v;
 }
 
+// What the rounding in join() left off, rounded in its turn.
+template <typename T>
+__device__ __forceinline__ Vec8<T> join_left(Vec8<T> rounded, f32x4 a, f32x4 b) {
+    Vec8<T> v;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        v[j] = static_cast<T>(a[j] - static_cast<float>(rounded[j]));
+        v[4 + j] = static_cast<T>(b[j] - static_cast<float>(rounded[4 + j]));
+    }
+    return v;
+}
+
 // Rows of a packed block: [first, first + count), never past the tensor.
 struct Rows {
     int64_t first;
@@ -161,12 +173,13 @@ struct AttendArgs {
     const int32_t* k_cells = nullptr;
     int axes = 0, buckets = 0, reach = 0;
     void* out = nullptr;   // (q_total, heads, D)
-    float* lse = nullptr;  // (q_total, heads), base 2; null: not wanted
+    float* lse = nullptr;  // (heads, q_total), base 2; null: not wanted
+    void* rest = nullptr;  // like out: what out's rounding left off (bf16 with a bias); null: not wanted
 };
 
 struct AttendGrads {
     const void* grad = nullptr;   // (q_total, heads, D) like out
-    float* delta = nullptr;       // (q_total, heads)
+    float* delta = nullptr;       // (heads, q_total)
     const uint32_t* keys = nullptr;   // sorted block numbers of the (group, slot) entries
     const int64_t* order = nullptr;   // their entries
     const int32_t* runs = nullptr;    // (blocks + 1) first sorted entry of each block
@@ -178,9 +191,7 @@ struct AttendGrads {
     int parts = 0;
 };
 
-// Bins of the table's gradient that one head may have: each has 64 copies in
-// LDS, one a lane, so that no two lanes add to one word and the order of the
-// additions is fixed.
+// Buckets that one head's table may have over all axes.
 constexpr int kMaxBins = 256;
 // Entries of one head's table expanded over all distances.
 constexpr int kMaxReachEntries = 4096;
@@ -213,7 +224,7 @@ __device__ __forceinline__ float across_groups_sum(float v) {
 
 // Cells are held as byte offsets into a table of floats, and far ones at the ends
 // of a range whose differences cannot overflow.
-constexpr int kFarCell = (1 << 28) - 1;
+constexpr int kFarCell = 1 << 26;
 __device__ __forceinline__ int cell_bytes(int cell) { return min(max(cell, -kFarCell), kFarCell) * 4; }
 // The distance of two such cells, clamped to [-reach, reach] (in bytes).
 __device__ __forceinline__ int cell_distance(int a, int b, int reach) { return min(max(a - b, -reach), reach); }

@@ -17,14 +17,50 @@ constexpr int kStep = 32;  // rows of the other side per step
 
 // Work-groups of the query-side kernel with a bias: each takes many tiles of one
 // head, so that few parts of the table's gradient are left to add up.
-constexpr int kTableParts = 192;  // per head, at most
+constexpr int kTableParts = 256;  // per head, at most
+
+// Smallest value of the lanes of `todo` (32 lanes' bits; the wave's two halves
+// hold the same), on every lane.
+__device__ __forceinline__ int least_of(int v, uint32_t todo) {
+    v = todo >> (lane_id() & 31) & 1u ? v : INT32_MAX;
+    v = min(v, __builtin_amdgcn_update_dpp(v, v, 0x128, 0xf, 0xf, false));  // rows of 16 rotated by 8, 4, 2, 1
+    v = min(v, __builtin_amdgcn_update_dpp(v, v, 0x124, 0xf, 0xf, false));
+    v = min(v, __builtin_amdgcn_update_dpp(v, v, 0x122, 0xf, 0xf, false));
+    v = min(v, __builtin_amdgcn_update_dpp(v, v, 0x121, 0xf, 0xf, false));
+    return min(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16));
+}
+
+// Unit vectors as a fragment: slot j is 1 where row j's cell is `at`.
+template <typename T>
+__device__ __forceinline__ Vec8<T> units(const int* cells, int g, int at) {
+    const int4 a = *reinterpret_cast<const int4*>(cells + 4 * g), b = *reinterpret_cast<const int4*>(cells + 16 + 4 * g);
+    const int c[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    Vec8<T> u;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) u[j] = static_cast<T>(c[j] == at ? 1.0f : 0.0f);
+    return u;
+}
+
+// The table's gradient on an axis is, distance by distance, a sum over the pairs
+// of cells that far apart: with unit vectors e of the cells, seen through windows of
+// 16 cells of either side, the 16 x 16 sums G = sum_ij e(cq_i) ds_ij e(ck_j)^T are
+// two more products, and only G's 256 entries are added in LDS, four a lane, instead
+// of the step's every ds (adding each one took 193 cycles a wave instruction as an
+// LDS float atomic, 10.5 of 12 ms of a training step over 80,000 points).  Cells of a
+// block of neighbours mostly fit one window; more windows are taken as needed.
+constexpr int kWindow = 16;
 
 // One wave per (tile of RT * 16 rows of a row block, head), or, with a bias, per
 // list of them: tiles part, part + parts, ... of one head.
 template <typename T, int DP, int RT, bool kBias>
-__global__ __launch_bounds__(kWave) void attend_dq_kernel(AttendArgs a, AttendGrads gr, int tiles, int64_t items) {
-    constexpr int DS = DP / 32, DT = DP / 16, KT = kStep / 16;
-    constexpr int LD = DP + 16 / sizeof(T);
+__global__ __launch_bounds__(kWave)
+    __attribute__((amdgpu_waves_per_eu(DP * RT * sizeof(T) > 512 || DP * sizeof(T) == 512 ? 1 : 2))) void attend_dq_kernel(AttendArgs a,
+                                                                                                  AttendGrads gr,
+                                                                                                  int tiles,
+                                                                                                  int64_t items) {
+    constexpr int DS = DP / 32, DT = DP / 16, KT = kStep / 16, E = sizeof(T);
+    constexpr int LD = turned_stride<T>(DP);
+    constexpr int kPairs = (RT + 1) / 2, kQueries = 32 * kPairs;  // row tiles in twos
     extern __shared__ float4 s_raw[];
     const int lane = lane_id(), n = lane & 15, g = lane >> 4;
     const int64_t item = xcd_item(blockIdx.x, gridDim.x);
@@ -34,36 +70,46 @@ __global__ __launch_bounds__(kWave) void attend_dq_kernel(AttendArgs a, AttendGr
     const int64_t all_tiles = static_cast<int64_t>(a.groups) * tiles;
 
     T* s_k = reinterpret_cast<T*>(s_raw);
-    float* s_bias = reinterpret_cast<float*>(s_k + kStep * LD);
-    const int span = 2 * a.reach + 1, entries = a.axes * span, bins = a.axes * a.buckets;
-    int* s_bin = reinterpret_cast<int*>(s_bias + entries);
-    float* s_sum = reinterpret_cast<float*>(s_bin + entries);  // (bins, 64): a copy a lane
+    int* s_cell = reinterpret_cast<int*>(s_k + kStep * LD);  // (3, 32) of the keys
+    int* s_query = s_cell + 3 * kStep;                       // (3, kQueries) of the queries
+    const int span = 2 * a.reach + 1, entries = a.axes * span, bins = a.axes * a.buckets, reach = 4 * a.reach;
+    float* s_bias = reinterpret_cast<float*>(s_query + 3 * kQueries);
+    // Sums by distance, -(reach + 31) to reach + 31, a copy for each g: the lanes of
+    // one copy always add at different distances.
+    const int wide = 2 * (a.reach + 2 * kWindow) - 1;
+    float* s_sum = s_bias + entries;  // (axes, 4, wide)
     if constexpr (kBias) {
         const T* table = static_cast<const T*>(a.table);
         for (int e = lane; e < entries; e += kWave) {
             const int axis = e / span;
             const int bin = axis * a.buckets + min(max(a.map[e - axis * span], 0), a.buckets - 1);
             s_bias[e] = static_cast<float>(table[bin * a.heads + h]) * kLog2e;
-            s_bin[e] = bin * kWave;
         }
-        for (int i = 0; i < bins; ++i) s_sum[i * kWave + lane] = 0.0f;
-        wave_sync();
+        for (int i = lane; i < a.axes * 4 * wide; i += kWave) s_sum[i] = 0.0f;
     }
     const float to_log2 = a.scale * kLog2e;
+    uint32_t k_at[KT][DS], v_at[KT][DS];
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int s = 0; s < DS; ++s) {
+            const int d = 32 * s + 8 * g;
+            k_at[kt][s] = d < a.D ? static_cast<uint32_t>((16 * kt + n) * a.k_row + d) * E : kNowhere;
+            v_at[kt][s] = d < a.D ? static_cast<uint32_t>((16 * kt + n) * a.v_row + d) * E : kNowhere;
+        }
 
     for (int64_t at = first; at < all_tiles; at += kBias ? gr.parts : all_tiles) {
         const int tile = static_cast<int>(at % tiles);
         const int64_t group = at / tiles;
         const Rows qr = block_rows(a.q_starts, group, a.q_block, a.q_total);
-        if (tile * RT * 16 >= qr.count) continue;
+        const int here = qr.count - tile * RT * 16;  // rows of the tile
+        if (here <= 0) continue;
         Vec8<T> qf[RT][DS], gf[RT][DS];
-        int qc[RT][3];
         float lse[RT], delta[RT];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-            const int rr = tile * RT * 16 + rt * 16 + n;
-            const bool real = rr < qr.count;
-            const int64_t row = qr.first + (real ? rr : 0);
+            const bool real = rt * 16 + n < here;
+            const int64_t row = qr.first + tile * RT * 16 + (real ? rt * 16 + n : 0);
             const T* qrow = static_cast<const T*>(a.q) + row * a.q_row + h * a.q_head;
             const T* grow = static_cast<const T*>(gr.grad) + (row * a.heads + h) * a.D;
             const T* orow = static_cast<const T*>(a.out) + (row * a.heads + h) * a.D;
@@ -76,13 +122,25 @@ __global__ __launch_bounds__(kWave) void attend_dq_kernel(AttendArgs a, AttendGr
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
                     dot = __builtin_fmaf(static_cast<float>(gf[rt][s][j]), static_cast<float>(o[j]), dot);
-            }
-            delta[rt] = across_groups_sum(dot);
-            lse[rt] = a.lse[row * a.heads + h];
-            if (real && g == 0) gr.delta[row * a.heads + h] = delta[rt];
-            if constexpr (kBias) {
+                if (kBias && a.rest != nullptr) {
+                    const Vec8<T> left = load8(static_cast<const T*>(a.rest) + (row * a.heads + h) * a.D, 32 * s + 8 * g,
+                                               a.D, real);
 #pragma unroll
-                for (int x = 0; x < 3; ++x) qc[rt][x] = x < a.axes ? cell_bytes(a.q_cells[row * a.axes + x]) : 0;
+                    for (int j = 0; j < 8; ++j)
+                        dot = __builtin_fmaf(static_cast<float>(gf[rt][s][j]), static_cast<float>(left[j]), dot);
+                }
+            }
+            // A row that is not there has q = grad = 0: ds is 0 whatever its weight.
+            delta[rt] = across_groups_sum(dot);
+            lse[rt] = real ? a.lse[h * a.q_total + row] : 0.0f;
+            if (real && g == 0) gr.delta[h * a.q_total + row] = delta[rt];
+        }
+        if constexpr (kBias) {
+            wave_sync();
+            for (int i = lane; i < a.axes * kQueries; i += kWave) {
+                const int x = i / kQueries, q = i - x * kQueries;
+                const int64_t row = qr.first + tile * RT * 16 + (q < here ? q : 0);
+                s_query[i] = cell_bytes(a.q_cells[row * a.axes + x]);
             }
         }
         f32x4 acc[RT][DT];
@@ -91,97 +149,183 @@ __global__ __launch_bounds__(kWave) void attend_dq_kernel(AttendArgs a, AttendGr
 #pragma unroll
             for (int t = 0; t < DT; ++t) acc[rt][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-        for (int slot = 0; slot < a.count; ++slot) {
-            const int block = __builtin_amdgcn_readfirstlane(a.selected[group * a.count + slot]);
-            if (block < 0 || block >= a.blocks) continue;
-            const Rows kr = block_rows(a.k_starts, block, a.k_block, a.k_total);
-            for (int base = 0; base < kr.count; base += kStep) {
-                const T* k0 = static_cast<const T*>(a.k) + (kr.first + base) * a.k_row + c * a.k_head;
-                const T* v0 = static_cast<const T*>(a.v) + (kr.first + base) * a.v_row + c * a.v_head;
-                const int left = kr.count - base;
-                f32x4 ds[KT][RT];
-                wave_sync();
+        for (int from = 0; from < a.count; from += kWave) {
+            const int slots = min(a.count - from, kWave);
+            Slots list;
+            list.load(a.selected + group * a.count + from, slots, a.blocks, a.k_starts, a.k_block, a.k_total);
+            int slot = 0, base = 0;
+            Rows kr = {0, 0};
+            const auto skip = [&] {
+                kr.count = 0;
+                while (slot < slots && (kr = list.at(slot)).count == 0) ++slot;
+            };
+            Vec8<T> kf[KT][DS], vf[KT][DS];
+            int cells[3];
+            const auto load = [&] {
+                const Buffer kb = rows_buffer<T>(a.k, kr.first + base, c * a.k_head, kr.count - base, a.k_row, a.D);
+                const Buffer vb = rows_buffer<T>(a.v, kr.first + base, c * a.v_head, kr.count - base, a.v_row, a.D);
 #pragma unroll
-                for (int kt = 0; kt < KT; ++kt) {
-                    const int row = 16 * kt + n;
-                    Vec8<T> kf[DS], vf[DS];
+                for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
                     for (int s = 0; s < DS; ++s) {
-                        kf[s] = load8(k0 + row * a.k_row, 32 * s + 8 * g, a.D, row < left);
-                        vf[s] = load8(v0 + row * a.v_row, 32 * s + 8 * g, a.D, row < left);
-                        *reinterpret_cast<Vec8<T>*>(s_k + row * LD + 32 * s + 8 * g) = kf[s];
+                        kf[kt][s] = load8<T>(kb, k_at[kt][s]);
+                        vf[kt][s] = load8<T>(vb, v_at[kt][s]);
                     }
-                    f32x4 st[RT];
+                if constexpr (kBias) {
+                    const int64_t row = kr.first + base + min(lane & (kStep - 1), max(kr.count - base - 1, 0));
+#pragma unroll
+                    for (int x = 0; x < 3; ++x)
+                        if (x < a.axes) cells[x] = a.k_cells[row * a.axes + x];
+                }
+            };
+            skip();
+            if (slot < slots) load();
+            while (slot < slots) {
+                const int left = kr.count - base;
+                wave_sync();
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                    for (int s = 0; s < DS; ++s)
+                        *reinterpret_cast<Vec8<T>*>(s_k + (16 * kt + n) * LD + 32 * s + 8 * g) = kf[kt][s];
+                if constexpr (kBias) {
+#pragma unroll
+                    for (int x = 0; x < 3; ++x)
+                        if (x < a.axes) s_cell[x * kStep + (lane & (kStep - 1))] = cell_bytes(cells[x]);
+                }
+                wave_sync();
+                f32x4 st[KT][RT], ds[KT][RT];
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
                     for (int rt = 0; rt < RT; ++rt) {
-                        f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+                        st[kt][rt] = ds[kt][rt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                        for (int s = 0; s < DS; ++s) x = mma(kf[s], qf[rt][s], x);
-                        st[rt] = x * to_log2;
+                        for (int s = 0; s < DS; ++s) {
+                            st[kt][rt] = mma(kf[kt][s], qf[rt][s], st[kt][rt]);
+                            ds[kt][rt] = mma(vf[kt][s], gf[rt][s], ds[kt][rt]);
+                        }
                     }
-                    if constexpr (kBias) {
-                        for (int x = 0; x < a.axes; ++x) {
+                base += kStep;
+                if (base >= kr.count) {
+                    base = 0;
+                    ++slot;
+                    skip();
+                }
+                if (slot < slots) load();
 #pragma unroll
-                            for (int r = 0; r < 4; ++r) {
-                                const int key = min(16 * kt + 4 * g + r, left - 1);
-                                const int kc = cell_bytes(a.k_cells[(kr.first + base + key) * a.axes + x]);
+                for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-                                for (int rt = 0; rt < RT; ++rt) {
-                                    const int q = x == 0 ? qc[rt][0] : x == 1 ? qc[rt][1] : qc[rt][2];
-                                    st[rt][r] += s_bias[x * span + a.reach + cell_distance(q, kc, 4 * a.reach) / 4];
-                                }
+                    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) st[kt][rt][r] = __builtin_fmaf(st[kt][rt][r], to_log2, -lse[rt]);
+                if constexpr (kBias) {
+#pragma unroll 1
+                    for (int x = 0; x < a.axes; ++x) {
+                        const char* table = reinterpret_cast<const char*>(s_bias + x * span + a.reach);
+                        int q[RT];
+#pragma unroll
+                        for (int rt = 0; rt < RT; ++rt) q[rt] = s_query[x * kQueries + 16 * rt + n];
+#pragma unroll
+                        for (int kt = 0; kt < KT; ++kt) {
+                            const int4 kc = *reinterpret_cast<const int4*>(s_cell + x * kStep + 16 * kt + 4 * g);
+                            const int key[4] = {kc.x, kc.y, kc.z, kc.w};
+#pragma unroll
+                            for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                                for (int r = 0; r < 4; ++r)
+                                    st[kt][rt][r] +=
+                                        *reinterpret_cast<const float*>(table + cell_distance(q[rt], key[r], reach));
+                        }
+                    }
+                }
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            ds[kt][rt][r] = __builtin_amdgcn_exp2f(st[kt][rt][r]) * (ds[kt][rt][r] - delta[rt]);
+                if (left < kStep) {
+#pragma unroll
+                    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (16 * kt + 4 * g + r >= left)
+#pragma unroll
+                                for (int rt = 0; rt < RT; ++rt) ds[kt][rt][r] = 0.0f;
+                }
+                // ds is rounded to T for the product with k; the table's sums, in which the
+                // terms of a row cancel, also take what that leaves off.
+                Vec8<T> df[RT], dl[RT];
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    df[rt] = join<T>(ds[0][rt], ds[1][rt]);
+                    if constexpr (kBias && E == 2) dl[rt] = join_left<T>(df[rt], ds[0][rt], ds[1][rt]);
+                }
+                if constexpr (kBias) {
+#pragma unroll 1
+                    for (int x = 0; x < a.axes; ++x) {
+                        const int key = s_cell[x * kStep + (lane & (kStep - 1))];
+                        uint32_t keys = static_cast<uint32_t>(__ballot((lane & (kStep - 1)) < left));
+                        while (keys != 0) {
+                            const int k_low = least_of(key, keys);
+                            keys &= ~static_cast<uint32_t>(__ballot(static_cast<uint32_t>(key - k_low) < 4 * kWindow));
+                            const Vec8<T> ku = units<T>(s_cell + x * kStep, g, k_low + 4 * n);
+                            f32x4 by_key[2 * kPairs];
+#pragma unroll
+                            for (int rt = 0; rt < 2 * kPairs; ++rt) {
+                                by_key[rt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                                if (rt < RT) by_key[rt] = mma(df[rt], ku, by_key[rt]);
+                                if (E == 2 && rt < RT) by_key[rt] = mma(dl[rt], ku, by_key[rt]);
                             }
-                        }
-                    }
+                            Vec8<T> part[kPairs], part_left[kPairs];
 #pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) {
-                        f32x4 dp = {0.0f, 0.0f, 0.0f, 0.0f};
+                            for (int p = 0; p < kPairs; ++p) {
+                                part[p] = join<T>(by_key[2 * p], by_key[2 * p + 1]);
+                                if constexpr (E == 2) part_left[p] = join_left<T>(part[p], by_key[2 * p], by_key[2 * p + 1]);
+                            }
+                            uint64_t rows = ~uint64_t{0} >> (64 - min(here, RT * 16));
+                            const int query = s_query[x * kQueries + (lane & (kQueries - 1))];
+                            while (rows != 0) {
+                                int q_low = least_of(query, static_cast<uint32_t>(rows));
+                                if (kPairs == 2) {
+                                    const int other = s_query[x * kQueries + ((lane + 32) & (kQueries - 1))];
+                                    const int up = least_of(lane < 32 ? other : query, static_cast<uint32_t>(rows >> 32));
+                                    q_low = min(least_of(lane < 32 ? query : other, static_cast<uint32_t>(rows)), up);
+                                }
+                                rows &= ~__ballot(static_cast<uint32_t>(query - q_low) < 4 * kWindow);
+                                f32x4 sums = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                        for (int s = 0; s < DS; ++s) dp = mma(vf[s], gf[rt][s], dp);
-                        const bool real = tile * RT * 16 + rt * 16 + n < qr.count;
+                                for (int p = 0; p < kPairs; ++p) {
+                                    const Vec8<T> qu = units<T>(s_query + x * kQueries + 32 * p, g, q_low + 4 * n);
+                                    sums = mma(qu, part[p], sums);
+                                    if constexpr (E == 2) sums = mma(qu, part_left[p], sums);
+                                }
+                                // sums[r]: query cell q_low + 4 g + r, key cell k_low + n.
+                                const int apart = min(max((q_low - k_low) / 4, -(a.reach + kWindow)), a.reach + kWindow);
+                                float* to = s_sum + (x * 4 + g) * wide + apart + a.reach + 2 * kWindow - 1 + 4 * g - n;
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const float p = __builtin_amdgcn_exp2f(st[rt][r] - lse[rt]);
-                            const bool in = real && 16 * kt + 4 * g + r < left;
-                            ds[kt][rt][r] = in ? p * (dp[r] - delta[rt]) : 0.0f;
-                        }
-                    }
-                    if constexpr (kBias) {
-                        for (int x = 0; x < a.axes; ++x) {
-#pragma unroll
-                            for (int r = 0; r < 4; ++r) {
-                                const int key = min(16 * kt + 4 * g + r, left - 1);
-                                const int kc = cell_bytes(a.k_cells[(kr.first + base + key) * a.axes + x]);
-#pragma unroll
-                                for (int rt = 0; rt < RT; ++rt) {
-                                    const int q = x == 0 ? qc[rt][0] : x == 1 ? qc[rt][1] : qc[rt][2];
-                                    float* bin = s_sum + s_bin[x * span + a.reach + cell_distance(q, kc, 4 * a.reach) / 4] + lane;
-                                    *bin += ds[kt][rt][r];
+                                for (int r = 0; r < 4; ++r) {
+                                    to[r] += sums[r];
+                                    wave_sync();
                                 }
                             }
                         }
                     }
                 }
-                wave_sync();
-                // ds is rounded to T for the product with k.
-                Vec8<T> df[RT];
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) df[rt] = join<T>(ds[0][rt], ds[1][rt]);
 #pragma unroll
                 for (int t = 0; t < DT; ++t) {
-                    Vec8<T> kf;
+                    const Vec8<T> kt = load_turned<T, LD>(s_k, t, n, g);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) kf[j] = s_k[(16 * (j / 4) + 4 * g + j % 4) * LD + 16 * t + n];
-#pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) acc[rt][t] = mma(kf, df[rt], acc[rt][t]);
+                    for (int rt = 0; rt < RT; ++rt) acc[rt][t] = mma(kt, df[rt], acc[rt][t]);
                 }
             }
         }
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-            const int rr = tile * RT * 16 + rt * 16 + n;
-            if (rr >= qr.count) continue;
-            T* row = static_cast<T*>(gr.dq) + ((qr.first + rr) * a.heads + h) * a.D;
+            if (rt * 16 + n >= here) continue;
+            T* row = static_cast<T*>(gr.dq) + ((qr.first + tile * RT * 16 + rt * 16 + n) * a.heads + h) * a.D;
 #pragma unroll
             for (int t = 0; t < DT; ++t) {
                 const int d = 16 * t + 4 * g;
@@ -198,9 +342,13 @@ __global__ __launch_bounds__(kWave) void attend_dq_kernel(AttendArgs a, AttendGr
         wave_sync();
         float* part = gr.table_parts + (first * a.heads + h) * bins;
         for (int b = lane; b < bins; b += kWave) {
+            const int axis = b / a.buckets;
             float total = 0.0f;
-            // Lane b starts at its own copy: 64 banks apart from its neighbours'.
-            for (int i = 0; i < kWave; ++i) total += s_sum[b * kWave + ((i + b) & (kWave - 1))];
+            for (int i = 0; i < wide; ++i) {
+                const int distance = min(max(i - a.reach - 2 * kWindow + 1, -a.reach), a.reach);
+                if (min(max(a.map[distance + a.reach], 0), a.buckets - 1) != b - axis * a.buckets) continue;
+                for (int copy = 0; copy < 4; ++copy) total += s_sum[(axis * 4 + copy) * wide + i];
+            }
             part[b] = total;
         }
     }
@@ -218,13 +366,19 @@ __global__ __launch_bounds__(kWave) void table_sum_kernel(const float* __restric
     if (lane_id() == 0) out[b * heads + h] = static_cast<T>(total);
 }
 
-// One wave per (32 rows of a key block, key head).  The rows of every chosen
-// row block's queries, for every head that shares the key head, are taken as one
-// list, 32 at a time.
-template <typename T, int DP, bool kBias>
-__global__ __launch_bounds__(kWave) void attend_dkv_kernel(AttendArgs a, AttendGrads gr, int tiles, int64_t items) {
-    constexpr int DS = DP / 32, DT = DP / 16, KT = 2, RT = kStep / 16;
-    constexpr int LD = DP + 16 / sizeof(T);
+// Tiles of 16 keys of a wave: two, or one where the registers hold no more.
+template <typename T>
+constexpr int key_tiles(int DP) { return sizeof(T) == 4 && DP == 128 ? 1 : 2; }
+
+// One wave per (KT * 16 rows of a key block, key head): the rows of every row block
+// that chose it, for every head that shares the key head, 32 at a time.  With
+// blocks of whole steps (kWhole) a step's rows are neighbours in one row block;
+// otherwise the blocks' rows are strung together and each lane finds its own.
+template <typename T, int DP, bool kBias, bool kWhole>
+__global__ __launch_bounds__(kWave) __attribute__((amdgpu_waves_per_eu(DP * sizeof(T) <= 128 ? 2 : 1))) void attend_dkv_kernel(
+    AttendArgs a, AttendGrads gr, int tiles, int64_t items) {
+    constexpr int DS = DP / 32, DT = DP / 16, KT = key_tiles<T>(DP), RT = kStep / 16, E = sizeof(T);
+    constexpr int LD = turned_stride<T>(DP);
     extern __shared__ float4 s_raw[];
     const int lane = lane_id(), n = lane & 15, g = lane >> 4;
     const int64_t item = xcd_item(blockIdx.x, gridDim.x);
@@ -238,12 +392,12 @@ __global__ __launch_bounds__(kWave) void attend_dkv_kernel(AttendArgs a, AttendG
 
     T* s_q = reinterpret_cast<T*>(s_raw);
     T* s_g = s_q + kStep * LD;
-    float* s_lse = reinterpret_cast<float*>(s_g + kStep * LD);
+    int* s_cell = reinterpret_cast<int*>(s_g + kStep * LD);  // (3, 32)
+    int* s_head = s_cell + 3 * kStep;                        // byte offset of the row's head's table
+    float* s_lse = reinterpret_cast<float*>(s_head + kStep);
     float* s_delta = s_lse + kStep;
-    int* s_cell = reinterpret_cast<int*>(s_delta + kStep);  // (3, 32)
-    int* s_head = s_cell + 3 * kStep;
-    float* s_bias = reinterpret_cast<float*>(s_head + kStep);
-    const int span = 2 * a.reach + 1, entries = a.axes * span;
+    float* s_bias = s_delta + kStep;
+    const int span = 2 * a.reach + 1, entries = a.axes * span, reach = 4 * a.reach;
     if constexpr (kBias) {
         const T* table = static_cast<const T*>(a.table);
         for (int i = lane; i < a.share * entries; i += kWave) {
@@ -254,19 +408,23 @@ __global__ __launch_bounds__(kWave) void attend_dkv_kernel(AttendArgs a, AttendG
     }
     Vec8<T> kf[KT][DS], vf[KT][DS];
     int kc[KT][3];
+    {
+        const Buffer kb = rows_buffer<T>(a.k, kr.first + base, c * a.k_head, left, a.k_row, a.D);
+        const Buffer vb = rows_buffer<T>(a.v, kr.first + base, c * a.v_head, left, a.v_row, a.D);
 #pragma unroll
-    for (int kt = 0; kt < KT; ++kt) {
-        const int row = 16 * kt + n;
-        const bool real = row < left;
-        const int64_t at = kr.first + base + (real ? row : 0);
+        for (int kt = 0; kt < KT; ++kt) {
+            const int row = 16 * kt + n;
 #pragma unroll
-        for (int s = 0; s < DS; ++s) {
-            kf[kt][s] = load8(static_cast<const T*>(a.k) + at * a.k_row + c * a.k_head, 32 * s + 8 * g, a.D, real);
-            vf[kt][s] = load8(static_cast<const T*>(a.v) + at * a.v_row + c * a.v_head, 32 * s + 8 * g, a.D, real);
-        }
-        if constexpr (kBias) {
+            for (int s = 0; s < DS; ++s) {
+                const int d = 32 * s + 8 * g;
+                kf[kt][s] = load8<T>(kb, d < a.D ? static_cast<uint32_t>(row * a.k_row + d) * E : kNowhere);
+                vf[kt][s] = load8<T>(vb, d < a.D ? static_cast<uint32_t>(row * a.v_row + d) * E : kNowhere);
+            }
+            if constexpr (kBias) {
+                const int64_t at = kr.first + base + min(row, left - 1);
 #pragma unroll
-            for (int x = 0; x < 3; ++x) kc[kt][x] = x < a.axes ? cell_bytes(a.k_cells[at * a.axes + x]) : 0;
+                for (int x = 0; x < 3; ++x) kc[kt][x] = x < a.axes ? cell_bytes(a.k_cells[at * a.axes + x]) : 0;
+            }
         }
     }
     f32x4 dk[KT][DT], dv[KT][DT];
@@ -275,96 +433,169 @@ __global__ __launch_bounds__(kWave) void attend_dkv_kernel(AttendArgs a, AttendG
 #pragma unroll
         for (int t = 0; t < DT; ++t) dk[kt][t] = dv[kt][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     const float to_log2 = a.scale * kLog2e;
-
-    const int run = gr.runs[block];
-    const int per = a.q_block * a.share;
-    const int64_t list = static_cast<int64_t>(gr.runs[block + 1] - run) * per;
-    for (int64_t v0 = 0; v0 < list; v0 += kStep) {
-        // Lane l < 32 finds row l of the step and leaves its values in LDS.
-        Vec8<T> qf[RT][DS], gf[RT][DS];
-        wave_sync();
+    const int64_t g_row = static_cast<int64_t>(a.heads) * a.D;
+    uint32_t q_at[RT][DS], g_at[RT][DS];
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            const int64_t v = v0 + 16 * rt + n;
-            const int64_t slot = v / per;
-            const int rr = static_cast<int>(v - slot * per);
-            const int qi = rr / a.share, hs = rr - qi * a.share;
-            bool real = v < list;
-            int64_t row = 0;
-            if (real) {
-                const Rows qr = block_rows(a.q_starts, gr.order[run + slot] / a.count, a.q_block, a.q_total);
-                real = qi < qr.count;
-                row = qr.first + (real ? qi : 0);
-            }
-            const int h = c * a.share + hs;
-            const T* qrow = static_cast<const T*>(a.q) + row * a.q_row + h * a.q_head;
-            const T* grow = static_cast<const T*>(gr.grad) + (row * a.heads + h) * a.D;
+    for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-            for (int s = 0; s < DS; ++s) {
-                qf[rt][s] = load8(qrow, 32 * s + 8 * g, a.D, real);
-                gf[rt][s] = load8(grow, 32 * s + 8 * g, a.D, real);
-                *reinterpret_cast<Vec8<T>*>(s_q + (16 * rt + n) * LD + 32 * s + 8 * g) = qf[rt][s];
-                *reinterpret_cast<Vec8<T>*>(s_g + (16 * rt + n) * LD + 32 * s + 8 * g) = gf[rt][s];
-            }
-            if (g == 0) {
-                // A row that is not there weighs nothing: exp2(s - inf) = 0.
-                s_lse[16 * rt + n] = real ? a.lse[row * a.heads + h] : INFINITY;
-                s_delta[16 * rt + n] = real ? gr.delta[row * a.heads + h] : 0.0f;
-                if constexpr (kBias) {
-                    s_head[16 * rt + n] = hs * entries;
-                    for (int x = 0; x < a.axes; ++x)
-                        s_cell[x * kStep + 16 * rt + n] = real ? cell_bytes(a.q_cells[row * a.axes + x]) : 0;
-                }
-            }
+        for (int s = 0; s < DS; ++s) {
+            const int d = 32 * s + 8 * g;
+            q_at[rt][s] = d < a.D ? static_cast<uint32_t>((16 * rt + n) * a.q_row + d) * E : kNowhere;
+            g_at[rt][s] = d < a.D ? static_cast<uint32_t>((16 * rt + n) * g_row + d) * E : kNowhere;
         }
-        wave_sync();
-        f32x4 p[RT][KT], ds[RT][KT];
+
+    const int run = gr.runs[block], run_end = gr.runs[block + 1];
+    const int per = a.q_block * a.share;
+    for (int from = run; from < run_end; from += kWave) {
+        // Lane i holds the rows of the run's i-th row block.
+        const int some = min(run_end - from, kWave);
+        Slots list = {0, 0, 0};
+        if (lane < some) {
+            const Rows r = block_rows(a.q_starts, gr.order[from + lane] / a.count, a.q_block, a.q_total);
+            list.first_lo = static_cast<int>(r.first);
+            list.first_hi = static_cast<int>(r.first >> 32);
+            list.count = r.count;
+        }
+        Vec8<T> qf[RT][DS], gf[RT][DS];
+        float lse = 0.0f, delta = 0.0f;
+        int cells[3] = {0, 0, 0}, head = 0;
+        const int steps = (some * per + kStep - 1) / kStep;
+        const auto load = [&](int step) {
+            if constexpr (kWhole) {
+                const int v = step * kStep, slot = v / per, rr = v - slot * per;
+                const int hs = rr / a.q_block, qi = rr - hs * a.q_block, h = c * a.share + hs;
+                const Rows qr = list.at(slot);
+                const int here = qr.count - qi;
+                const int64_t row = qr.first + qi;
+                const Buffer qb = rows_buffer<T>(a.q, row, h * a.q_head, here, a.q_row, a.D);
+                const Buffer gb = rows_buffer<T>(gr.grad, row, static_cast<int64_t>(h) * a.D, here, g_row, a.D);
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            const f32x4 lse = *reinterpret_cast<const f32x4*>(s_lse + 16 * rt + 4 * g);
-            const f32x4 delta = *reinterpret_cast<const f32x4*>(s_delta + 16 * rt + 4 * g);
+                for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-            for (int kt = 0; kt < KT; ++kt) {
-                f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f}, dp = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int s = 0; s < DS; ++s) {
-                    x = mma(qf[rt][s], kf[kt][s], x);
-                    dp = mma(gf[rt][s], vf[kt][s], dp);
-                }
-                x = x * to_log2;
+                    for (int s = 0; s < DS; ++s) {
+                        qf[rt][s] = load8<T>(qb, q_at[rt][s]);
+                        gf[rt][s] = load8<T>(gb, g_at[rt][s]);
+                    }
+                // Rows that are not there have q = grad = 0, so nothing comes of theirs.
+                const int64_t mine = min(max(row + min(lane & (kStep - 1), here - 1), int64_t{0}), a.q_total - 1);
+                lse = a.lse[h * a.q_total + mine];
+                delta = gr.delta[h * a.q_total + mine];
                 if constexpr (kBias) {
-                    for (int ax = 0; ax < a.axes; ++ax) {
-                        const int key = ax == 0 ? kc[kt][0] : ax == 1 ? kc[kt][1] : kc[kt][2];
+                    head = hs * entries * 4;
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const int q = 16 * rt + 4 * g + r;
-                            x[r] += s_bias[s_head[q] + ax * span + a.reach + cell_distance(s_cell[ax * kStep + q], key, 4 * a.reach) / 4];
-                        }
+                    for (int x = 0; x < 3; ++x)
+                        if (x < a.axes) cells[x] = a.q_cells[mine * a.axes + x];
+                }
+            } else {
+                const auto find = [&](int v, int& h, bool& real) -> int64_t {
+                    const int slot = v / per, rr = v - slot * per;
+                    const int hs = rr / a.q_block, qi = rr - hs * a.q_block;
+                    const uint32_t lo = __shfl(list.first_lo, slot & (kWave - 1), kWave);
+                    const int64_t hi = __shfl(list.first_hi, slot & (kWave - 1), kWave);
+                    const int count = __shfl(list.count, slot & (kWave - 1), kWave);
+                    h = c * a.share + hs;
+                    real = slot < some && qi < count;
+                    return real ? (hi << 32 | lo) + qi : 0;
+                };
+                int h;
+                bool real;
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    const int64_t row = find(step * kStep + 16 * rt + n, h, real);
+                    const T* qrow = static_cast<const T*>(a.q) + row * a.q_row + h * a.q_head;
+                    const T* grow = static_cast<const T*>(gr.grad) + row * g_row + static_cast<int64_t>(h) * a.D;
+#pragma unroll
+                    for (int s = 0; s < DS; ++s) {
+                        qf[rt][s] = load8(qrow, 32 * s + 8 * g, a.D, real);
+                        gf[rt][s] = load8(grow, 32 * s + 8 * g, a.D, real);
                     }
                 }
-                const bool in = 16 * kt + n < left;
+                const int64_t mine = find(step * kStep + (lane & (kStep - 1)), h, real);
+                lse = a.lse[h * a.q_total + mine];
+                delta = gr.delta[h * a.q_total + mine];
+                if constexpr (kBias) {
+                    head = (h - c * a.share) * entries * 4;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float w = lse[r] == INFINITY || !in ? 0.0f : __builtin_amdgcn_exp2f(x[r] - lse[r]);
-                    p[rt][kt][r] = w;
-                    ds[rt][kt][r] = lse[r] == INFINITY || !in ? 0.0f : w * (dp[r] - delta[r]);
+                    for (int x = 0; x < 3; ++x)
+                        if (x < a.axes) cells[x] = a.q_cells[mine * a.axes + x];
                 }
             }
-        }
+        };
+        load(0);
+        for (int step = 0; step < steps; ++step) {
+            wave_sync();
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt) {
-            const Vec8<T> pf = join<T>(p[0][kt], p[1][kt]), df = join<T>(ds[0][kt], ds[1][kt]);
+            for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-            for (int t = 0; t < DT; ++t) {
-                Vec8<T> gt, qt;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int at = (16 * (j / 4) + 4 * g + j % 4) * LD + 16 * t + n;
-                    gt[j] = s_g[at];
-                    qt[j] = s_q[at];
+                for (int s = 0; s < DS; ++s) {
+                    *reinterpret_cast<Vec8<T>*>(s_q + (16 * rt + n) * LD + 32 * s + 8 * g) = qf[rt][s];
+                    *reinterpret_cast<Vec8<T>*>(s_g + (16 * rt + n) * LD + 32 * s + 8 * g) = gf[rt][s];
                 }
-                dv[kt][t] = mma(gt, pf, dv[kt][t]);
-                dk[kt][t] = mma(qt, df, dk[kt][t]);
+            if (lane < kStep) {
+                s_lse[lane] = lse;
+                s_delta[lane] = delta;
+                if constexpr (kBias) {
+                    s_head[lane] = head;
+#pragma unroll
+                    for (int x = 0; x < 3; ++x)
+                        if (x < a.axes) s_cell[x * kStep + lane] = cell_bytes(cells[x]);
+                }
+            }
+            wave_sync();
+            f32x4 p[RT][KT], ds[RT][KT];
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) {
+                    p[rt][kt] = ds[rt][kt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int s = 0; s < DS; ++s) {
+                        p[rt][kt] = mma(qf[rt][s], kf[kt][s], p[rt][kt]);
+                        ds[rt][kt] = mma(gf[rt][s], vf[kt][s], ds[rt][kt]);
+                    }
+                }
+            if (step + 1 < steps) load(step + 1);
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                const f32x4 l = *reinterpret_cast<const f32x4*>(s_lse + 16 * rt + 4 * g);
+                const f32x4 dl = *reinterpret_cast<const f32x4*>(s_delta + 16 * rt + 4 * g);
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) p[rt][kt][r] = __builtin_fmaf(p[rt][kt][r], to_log2, -l[r]);
+                if constexpr (kBias) {
+                    const int4 hd = *reinterpret_cast<const int4*>(s_head + 16 * rt + 4 * g);
+                    const int heads[4] = {hd.x, hd.y, hd.z, hd.w};
+#pragma unroll
+                    for (int x = 0; x < 3; ++x) {
+                        if (x >= a.axes) continue;
+                        const int4 qc = *reinterpret_cast<const int4*>(s_cell + x * kStep + 16 * rt + 4 * g);
+                        const int q[4] = {qc.x, qc.y, qc.z, qc.w};
+                        const char* table = reinterpret_cast<const char*>(s_bias + x * span + a.reach);
+#pragma unroll
+                        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r)
+                                p[rt][kt][r] += *reinterpret_cast<const float*>(
+                                    table + heads[r] + cell_distance(q[r], kc[kt][x], reach));
+                    }
+                }
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        p[rt][kt][r] = __builtin_amdgcn_exp2f(p[rt][kt][r]);
+                        ds[rt][kt][r] = p[rt][kt][r] * (ds[rt][kt][r] - dl[r]);
+                    }
+            }
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) {
+                const Vec8<T> pf = join<T>(p[0][kt], p[1][kt]), df = join<T>(ds[0][kt], ds[1][kt]);
+#pragma unroll
+                for (int t = 0; t < DT; ++t) {
+                    dv[kt][t] = mma(load_turned<T, LD>(s_g, t, n, g), pf, dv[kt][t]);
+                    dk[kt][t] = mma(load_turned<T, LD>(s_q, t, n, g), df, dk[kt][t]);
+                }
             }
         }
     }
@@ -439,8 +670,9 @@ hipError_t launch_dq(const AttendArgs& a, const AttendGrads& g, hipStream_t stre
     const int tiles = (a.q_block + RT * 16 - 1) / (RT * 16);
     const int64_t items = (kBias ? g.parts : static_cast<int64_t>(a.groups) * tiles) * a.heads;
     const int entries = a.axes * (2 * a.reach + 1);
-    const size_t lds = kStep * (DP + 16 / sizeof(T)) * sizeof(T) +
-                       (kBias ? (entries * 2 + static_cast<size_t>(a.axes) * a.buckets * kWave) * sizeof(float) : 0);
+    const size_t lds = kStep * turned_stride<T>(DP) * sizeof(T) + 3 * (kStep + 32 * ((RT + 1) / 2)) * sizeof(int) +
+                       (kBias ? entries + static_cast<size_t>(a.axes) * 4 * (2 * (a.reach + 2 * kWindow) - 1) : 0) *
+                           sizeof(float);
     const auto kernel = attend_dq_kernel<T, DP, RT, kBias>;
     const hipError_t e = allow_lds(kernel, lds);
     if (e != hipSuccess) return e;
@@ -448,13 +680,14 @@ hipError_t launch_dq(const AttendArgs& a, const AttendGrads& g, hipStream_t stre
     return hipGetLastError();
 }
 
-template <typename T, int DP, bool kBias>
+template <typename T, int DP, bool kBias, bool kWhole>
 hipError_t launch_dkv(const AttendArgs& a, const AttendGrads& g, hipStream_t stream) {
-    const int tiles = (a.k_block + 31) / 32;
+    constexpr int kKeys = 16 * key_tiles<T>(DP);
+    const int tiles = (a.k_block + kKeys - 1) / kKeys;
     const int64_t items = static_cast<int64_t>(a.blocks) * tiles * a.kv_heads;
-    const size_t lds = 2 * kStep * (DP + 16 / sizeof(T)) * sizeof(T) + 6 * kStep * sizeof(float) +
+    const size_t lds = 2 * kStep * turned_stride<T>(DP) * sizeof(T) + 6 * kStep * sizeof(float) +
                        (kBias ? static_cast<size_t>(a.share) * a.axes * (2 * a.reach + 1) * sizeof(float) : 0);
-    const auto kernel = attend_dkv_kernel<T, DP, kBias>;
+    const auto kernel = attend_dkv_kernel<T, DP, kBias, kWhole>;
     const hipError_t e = allow_lds(kernel, lds);
     if (e != hipSuccess) return e;
     kernel<<<static_cast<unsigned>(xcd_grid(items)), kWave, lds, stream>>>(a, g, tiles, items);
@@ -474,7 +707,8 @@ hipError_t launch_pair(const AttendArgs& a, const AttendGrads& g, hipStream_t st
         e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
-    return launch_dkv<T, DP, kBias>(a, g, stream);
+    return a.q_block % kStep == 0 ? launch_dkv<T, DP, kBias, true>(a, g, stream)
+                                  : launch_dkv<T, DP, kBias, false>(a, g, stream);
 }
 
 template <typename T>

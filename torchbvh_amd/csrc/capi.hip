@@ -1570,16 +1570,19 @@ int check_attend(const char* op, const tbvh_attend_args* x, AttendArgs& a) {
     if (x->groups * std::max<int64_t>(x->count, 1) > kMaxRows) {
         return fail(TBVH_ERR_INVALID_ARGUMENT, "%s: groups * count must fit in signed int32", op);
     }
+    if (x->heads * int64_t{x->D} > kMaxRowStride) {
+        return fail(TBVH_ERR_INVALID_ARGUMENT, "%s: heads * D must be at most 2^21", op);
+    }
     const int64_t share = x->heads / x->kv_heads;
-    // Tiles have 16 rows at least; the backward's, 32 of a key block.
+    // Tiles have 16 rows at least; the backward's, 16 of a key block.
     if (x->groups * ((x->q_block * share + 15) / 16) > kMaxGroups / x->heads ||
-        x->blocks * 4 > kMaxGroups / x->heads) {
+        x->blocks * 8 > kMaxGroups / x->heads) {
         return fail(TBVH_ERR_INVALID_ARGUMENT, "%s: too many (block, head) pairs for one launch", op);
     }
     const int64_t strides = x->q_row_stride | x->q_head_stride | x->k_row_stride | x->k_head_stride | x->v_row_stride |
                             x->v_head_stride;
     if (strides * (x->bf16 ? 2 : 4) % 16 != 0 || !multiple_of_16(x->q) || !multiple_of_16(x->k) || !multiple_of_16(x->v) ||
-        !multiple_of_16(x->out)) {
+        !multiple_of_16(x->out) || !multiple_of_16(x->rest)) {
         return fail(TBVH_ERR_INVALID_ARGUMENT, "%s: q, k, v and out must be 16-byte aligned, and their strides", op);
     }
     // A block's rows are addressed with 31 bits.
@@ -1637,6 +1640,7 @@ int check_attend(const char* op, const tbvh_attend_args* x, AttendArgs& a) {
     a.reach = x->reach;
     a.out = x->out;
     a.lse = x->lse;
+    a.rest = x->bf16 && x->table ? x->rest : nullptr;
     return TBVH_OK;
 }
 
