@@ -62,12 +62,11 @@ __global__ __launch_bounds__(kWave* W) __attribute__((amdgpu_waves_per_eu(forwar
         __syncthreads();
     }
 
-    // Scores in powers of two are fma(s, to_log2, bias); a negative scale goes into
-    // the queries, so the largest score is the largest product.
-    const float to_log2 = fabsf(a.scale) * kLog2e;
+    const float to_log2 = a.scale * kLog2e;
     Vec8<T> qf[RT][DS];
-    int qc[RT][3];
-    const char* bias_row[RT];
+    int qc[RT][3];                           // cells of an axis, and at the row's table
+    int close_from[3] = {}, close_span[3] = {};  // key cells that no query's distance is clamped for
+    int bias_row[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         const int rr = tile * RT * 16 + rt * 16 + n;
@@ -75,30 +74,39 @@ __global__ __launch_bounds__(kWave* W) __attribute__((amdgpu_waves_per_eu(forwar
         const int qi = real ? rr / a.share : 0, hs = real ? rr - qi * a.share : 0;
         const T* row = static_cast<const T*>(a.q) + (qr.first + qi) * a.q_row + (c * a.share + hs) * a.q_head;
 #pragma unroll
-        for (int s = 0; s < DS; ++s) {
-            qf[rt][s] = load8(row, 32 * s + 8 * g, a.D, real);
-            if (a.scale < 0.0f) qf[rt][s] = -qf[rt][s];
-        }
+        for (int s = 0; s < DS; ++s) qf[rt][s] = load8(row, 32 * s + 8 * g, a.D, real);
         if constexpr (kBias) {
-            bias_row[rt] = reinterpret_cast<const char*>(s_bias + hs * entries + a.reach);
+            bias_row[rt] = (hs * entries + a.reach) * 4;
 #pragma unroll
             for (int x = 0; x < 3; ++x) qc[rt][x] = x < a.axes ? cell_bytes(a.q_cells[(qr.first + qi) * a.axes + x]) : 0;
         }
     }
+    if constexpr (kBias) {
+#pragma unroll
+        for (int x = 0; x < 3; ++x) {
+            int lo = qc[0][x], hi = qc[0][x];
+#pragma unroll
+            for (int rt = 1; rt < RT; ++rt) {
+                lo = min(lo, qc[rt][x]);
+                hi = max(hi, qc[rt][x]);
+            }
+            close_from[x] = largest_lane(hi) - reach;
+            close_span[x] = least_lane(lo) + reach - close_from[x];
+        }
+    }
 
     f32x4 acc[RT][DT], sums[RT];
-    float top[RT], sum[RT];
+    // Weights are exp2(score - ref); a score that exceeds ref by over `limit` moves it.
+    float ref[RT], limit[RT], sum[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-        top[rt] = -INFINITY;
+        ref[rt] = 0.0f;
+        limit[rt] = -INFINITY;  // no score yet: the first one sets it
         sum[rt] = 0.0f;
         sums[rt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int t = 0; t < DT; ++t) acc[rt][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    // A score in units of `unit` powers of two: with a bias they are converted first.
-    const float unit = kBias ? 1.0f : to_log2;
-    const float slack = unit > 0.0f ? kSlack / unit : 3.0e38f;
     // A table's gradient is a sum in which each row's scores cancel, down to the
     // error of delta = grad . out; so where it is wanted the weights take part with
     // what their rounding left off, too, and so is the output kept.
@@ -188,22 +196,39 @@ __global__ __launch_bounds__(kWave* W) __attribute__((amdgpu_waves_per_eu(forwar
                     for (int s = 0; s < DS; ++s) st[kt][rt] = mma(kf[kt][s], qf[rt][s], st[kt][rt]);
                 }
             if (slot < slots) load_keys();
+            // Scores less the reference, in powers of two.
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) st[kt][rt][r] = __builtin_fmaf(st[kt][rt][r], to_log2, -ref[rt]);
             if constexpr (kBias) {
 #pragma unroll
-                for (int kt = 0; kt < KT; ++kt) {
+                for (int x = 0; x < 3; ++x) {
+                    if (x >= a.axes) continue;
+                    const int mine = s_cell[x * kChunk + (lane & (kChunk - 1))];
+                    const bool close = __all(static_cast<uint32_t>(mine - close_from[x]) <= static_cast<uint32_t>(close_span[x])) &&
+                                       close_span[x] >= 0;
+                    const char* table = reinterpret_cast<const char*>(s_bias + x * span);
 #pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) st[kt][rt] *= to_log2;
-#pragma unroll
-                    for (int x = 0; x < 3; ++x) {
-                        if (x >= a.axes) continue;
+                    for (int kt = 0; kt < KT; ++kt) {
                         const int4 kc = *reinterpret_cast<const int4*>(s_cell + x * kChunk + 16 * kt + 4 * g);
                         const int key[4] = {kc.x, kc.y, kc.z, kc.w};
+                        if (close) {
 #pragma unroll
-                        for (int rt = 0; rt < RT; ++rt)
+                            for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-                            for (int r = 0; r < 4; ++r)
-                                st[kt][rt][r] += *reinterpret_cast<const float*>(
-                                    bias_row[rt] + x * span * 4 + cell_distance(qc[rt][x], key[r], reach));
+                                for (int r = 0; r < 4; ++r)
+                                    st[kt][rt][r] += *reinterpret_cast<const float*>(table + (bias_row[rt] + qc[rt][x] - key[r]));
+                        } else {
+#pragma unroll
+                            for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                                for (int r = 0; r < 4; ++r)
+                                    st[kt][rt][r] += *reinterpret_cast<const float*>(
+                                        table + (bias_row[rt] + cell_distance(qc[rt][x], key[r], reach)));
+                        }
                     }
                 }
             }
@@ -225,18 +250,26 @@ __global__ __launch_bounds__(kWave* W) __attribute__((amdgpu_waves_per_eu(forwar
                 for (int kt = 1; kt < KT; ++kt)
                     m = fmaxf(fmaxf(fmaxf(m, st[kt][rt][0]), fmaxf(st[kt][rt][1], st[kt][rt][2])), st[kt][rt][3]);
                 most[rt] = m;
-                above |= m > top[rt] + slack;
+                above |= m > limit[rt];
             }
             if (__any(above)) {
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) {
-                    const float m = fmaxf(top[rt], across_groups_max(most[rt]));
-                    const float keep = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((top[rt] - m) * unit);
-                    top[rt] = m;
+                    // The largest score so far, and how far the reference follows: rows that
+                    // have met no score above -inf keep a reference of 0 and weights of 0.
+                    const float m = across_groups_max(most[rt]);
+                    const float up = limit[rt] < 0.0f ? (m == -INFINITY ? 0.0f : m) : fmaxf(m, 0.0f);
+                    if (m != -INFINITY) limit[rt] = kSlack;
+                    const float keep = __builtin_amdgcn_exp2f(-up);
+                    ref[rt] += up;
                     sum[rt] *= keep;
                     sums[rt] *= keep;
 #pragma unroll
                     for (int t = 0; t < DT; ++t) acc[rt][t] *= keep;
+#pragma unroll
+                    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) st[kt][rt][r] -= up;
                 }
             }
             // Weights are rounded to T for the product with v (2^-9 each in bf16,
@@ -244,24 +277,10 @@ __global__ __launch_bounds__(kWave* W) __attribute__((amdgpu_waves_per_eu(forwar
             Vec8<T> pf[RT], lo[RT];
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
-                // Rows that have met no finite score yet keep weights of zero.
-                const float ref = top[rt] == -INFINITY ? 0.0f : -top[rt] * unit;
 #pragma unroll
                 for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        st[kt][rt][r] = __builtin_amdgcn_exp2f(kBias ? st[kt][rt][r] + ref
-                                                                     : __builtin_fmaf(st[kt][rt][r], unit, ref));
-            }
-            if (left < kChunk) {
-                // Not left to exp2(-inf): a scale of zero would make it undefined.
-#pragma unroll
-                for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (16 * kt + 4 * g + r >= left)
-#pragma unroll
-                            for (int rt = 0; rt < RT; ++rt) st[kt][rt][r] = 0.0f;
+                    for (int r = 0; r < 4; ++r) st[kt][rt][r] = __builtin_amdgcn_exp2f(st[kt][rt][r]);
             }
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
@@ -295,14 +314,14 @@ __global__ __launch_bounds__(kWave* W) __attribute__((amdgpu_waves_per_eu(forwar
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) sum[rt] = kSumByProduct ? sums[rt][0] : across_groups_sum(sum[rt]);
     if constexpr (W > 1) {
-        // Every wave's (top, sum, acc) through LDS; wave 0 joins them in order.
+        // Every wave's (ref, sum, acc) through LDS; wave 0 joins them in order.
         float* s_part = reinterpret_cast<float*>(s_raw);
         constexpr int kPer = RT * (DT * 4 + 2) * kWave;
         __syncthreads();
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             float* p = s_part + wave * kPer + rt * (DT * 4 + 2) * kWave + lane;
-            p[0] = top[rt];
+            p[0] = limit[rt] < 0.0f ? -INFINITY : ref[rt];
             p[kWave] = sum[rt];
 #pragma unroll
             for (int t = 0; t < DT; ++t)
@@ -314,12 +333,10 @@ __global__ __launch_bounds__(kWave* W) __attribute__((amdgpu_waves_per_eu(forwar
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             const float* p = s_part + rt * (DT * 4 + 2) * kWave + lane;
-            float m = top[rt];
+            float m = p[0];
             for (int w = 1; w < W; ++w) m = fmaxf(m, p[w * kPer]);
-            const auto weight = [&](float t) {
-                return t == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((t - m) * unit);
-            };
-            const float keep = weight(top[rt]);
+            const auto weight = [&](float t) { return t == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(t - m); };
+            const float keep = weight(p[0]);
             sum[rt] *= keep;
 #pragma unroll
             for (int t = 0; t < DT; ++t) acc[rt][t] *= keep;
@@ -331,7 +348,7 @@ __global__ __launch_bounds__(kWave* W) __attribute__((amdgpu_waves_per_eu(forwar
 #pragma unroll
                     for (int r = 0; r < 4; ++r) acc[rt][t][r] += p[w * kPer + (2 + t * 4 + r) * kWave] * f;
             }
-            top[rt] = m;
+            ref[rt] = m;
         }
     }
 
@@ -363,7 +380,7 @@ __global__ __launch_bounds__(kWave* W) __attribute__((amdgpu_waves_per_eu(forwar
         // 0 for an empty row: its scores are all -inf, their weights 0 again.
         if (a.lse != nullptr && g == 0)
             a.lse[(c * a.share + hs) * a.q_total + qr.first + qi] =
-                sum[rt] == 0.0f ? 0.0f : __builtin_fmaf(top[rt], unit, __builtin_amdgcn_logf(sum[rt]));
+                sum[rt] == 0.0f ? 0.0f : ref[rt] + __builtin_amdgcn_logf(sum[rt]);
     }
 }
 

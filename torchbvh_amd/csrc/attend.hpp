@@ -229,6 +229,17 @@ __device__ __forceinline__ int cell_bytes(int cell) { return min(max(cell, -kFar
 // The distance of two such cells, clamped to [-reach, reach] (in bytes).
 __device__ __forceinline__ int cell_distance(int a, int b, int reach) { return min(max(a - b, -reach), reach); }
 
+// Least and largest value of a wave's lanes, in scalar registers.
+__device__ __forceinline__ int least_lane(int v) {
+    v = min(v, __builtin_amdgcn_update_dpp(v, v, 0x128, 0xf, 0xf, false));  // rows of 16 rotated by 8, 4, 2, 1
+    v = min(v, __builtin_amdgcn_update_dpp(v, v, 0x124, 0xf, 0xf, false));
+    v = min(v, __builtin_amdgcn_update_dpp(v, v, 0x122, 0xf, 0xf, false));
+    v = min(v, __builtin_amdgcn_update_dpp(v, v, 0x121, 0xf, 0xf, false));
+    return min(min(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)),
+               min(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
+}
+__device__ __forceinline__ int largest_lane(int v) { return -least_lane(-v); }
+
 // The key blocks chosen for a row block, 64 slots at a time: lane i holds slot
 // i's rows, and walking them needs no further loads.
 struct Slots {
@@ -253,9 +264,10 @@ struct Slots {
 hipError_t launch_attend(const AttendArgs& a, bool bf16, hipStream_t stream);
 hipError_t launch_attend_backward(const AttendArgs& a, const AttendGrads& g, bool bf16, hipStream_t stream);
 // Parts of the table's gradient for these sizes.
-int attend_table_parts(int groups, int q_block, int heads);
+int attend_table_parts(const AttendArgs& a, bool bf16);
 
-// Inverse of a selection: the (group, slot) entries sorted by block.
+// Inverse of a selection: the (group, slot) entries sorted by block and each block's
+// run of them.
 hipError_t launch_invert(const int32_t* selected, int64_t entries, int blocks, Segment* segs, int64_t tiles,
                          const SortBuffers& sb, int64_t* order, int32_t* runs, hipStream_t stream);
 

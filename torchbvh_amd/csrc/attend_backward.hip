@@ -15,9 +15,14 @@ namespace {
 
 constexpr int kStep = 32;  // rows of the other side per step
 
-// Work-groups of the query-side kernel with a bias: each takes many tiles of one
-// head, so that few parts of the table's gradient are left to add up.
-constexpr int kTableParts = 256;  // per head, at most
+// Waves of the query-side kernel with a bias, over all heads: each takes many tiles
+// of one head, so that few parts of the table's gradient are left to add up.
+constexpr int kTableWaves = 2048;
+
+constexpr int64_t kSplitWaves = 1 << 16;
+
+// Tiles of 16 query rows of a wave.
+constexpr int query_tiles(int size, int DP, int q_block) { return q_block <= 16 ? 1 : size == 2 && DP <= 32 ? 4 : 2; }
 
 // Smallest value of the lanes of `todo` (32 lanes' bits; the wave's two halves
 // hold the same), on every lane.
@@ -73,7 +78,8 @@ __global__ __launch_bounds__(kWave)
     int* s_cell = reinterpret_cast<int*>(s_k + kStep * LD);  // (3, 32) of the keys
     int* s_query = s_cell + 3 * kStep;                       // (3, kQueries) of the queries
     const int span = 2 * a.reach + 1, entries = a.axes * span, bins = a.axes * a.buckets, reach = 4 * a.reach;
-    float* s_bias = reinterpret_cast<float*>(s_query + 3 * kQueries);
+    Vec8<T>* s_units = reinterpret_cast<Vec8<T>*>(s_query + 3 * kQueries);  // (3, kPairs, 64) of the queries' first window
+    float* s_bias = reinterpret_cast<float*>(s_units + 3 * kPairs * kWave);
     // Sums by distance, -(reach + 31) to reach + 31, a copy for each g: the lanes of
     // one copy always add at different distances.
     const int wide = 2 * (a.reach + 2 * kWindow) - 1;
@@ -106,6 +112,7 @@ __global__ __launch_bounds__(kWave)
         if (here <= 0) continue;
         Vec8<T> qf[RT][DS], gf[RT][DS];
         float lse[RT], delta[RT];
+        int q_least[3] = {}, q_most[3] = {};  // cells of the tile's queries
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             const bool real = rt * 16 + n < here;
@@ -141,6 +148,17 @@ __global__ __launch_bounds__(kWave)
                 const int x = i / kQueries, q = i - x * kQueries;
                 const int64_t row = qr.first + tile * RT * 16 + (q < here ? q : 0);
                 s_query[i] = cell_bytes(a.q_cells[row * a.axes + x]);
+            }
+            wave_sync();
+#pragma unroll
+            for (int x = 0; x < 3; ++x) {
+                if (x >= a.axes) continue;
+                const int q = s_query[x * kQueries + (lane & (kQueries - 1))];
+                q_least[x] = least_lane(q);
+                q_most[x] = largest_lane(q);
+#pragma unroll
+                for (int p = 0; p < kPairs; ++p)
+                    s_units[(x * kPairs + p) * kWave + lane] = units<T>(s_query + x * kQueries + 32 * p, g, q_least[x] + 4 * n);
             }
         }
         f32x4 acc[RT][DT];
@@ -220,9 +238,13 @@ __global__ __launch_bounds__(kWave)
 #pragma unroll
                         for (int r = 0; r < 4; ++r) st[kt][rt][r] = __builtin_fmaf(st[kt][rt][r], to_log2, -lse[rt]);
                 if constexpr (kBias) {
-#pragma unroll 1
-                    for (int x = 0; x < a.axes; ++x) {
+#pragma unroll
+                    for (int x = 0; x < 3; ++x) {
+                        if (x >= a.axes) continue;
                         const char* table = reinterpret_cast<const char*>(s_bias + x * span + a.reach);
+                        // Whether no distance of the step is clamped.
+                        const int mine = s_cell[x * kStep + (lane & (kStep - 1))];
+                        const bool close = __all(q_most[x] - mine <= reach && mine - q_least[x] <= reach);
                         int q[RT];
 #pragma unroll
                         for (int rt = 0; rt < RT; ++rt) q[rt] = s_query[x * kQueries + 16 * rt + n];
@@ -230,12 +252,20 @@ __global__ __launch_bounds__(kWave)
                         for (int kt = 0; kt < KT; ++kt) {
                             const int4 kc = *reinterpret_cast<const int4*>(s_cell + x * kStep + 16 * kt + 4 * g);
                             const int key[4] = {kc.x, kc.y, kc.z, kc.w};
+                            if (close) {
 #pragma unroll
-                            for (int rt = 0; rt < RT; ++rt)
+                                for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-                                for (int r = 0; r < 4; ++r)
-                                    st[kt][rt][r] +=
-                                        *reinterpret_cast<const float*>(table + cell_distance(q[rt], key[r], reach));
+                                    for (int r = 0; r < 4; ++r)
+                                        st[kt][rt][r] += *reinterpret_cast<const float*>(table + (q[rt] - key[r]));
+                            } else {
+#pragma unroll
+                                for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                                    for (int r = 0; r < 4; ++r)
+                                        st[kt][rt][r] +=
+                                            *reinterpret_cast<const float*>(table + cell_distance(q[rt], key[r], reach));
+                            }
                         }
                     }
                 }
@@ -264,12 +294,15 @@ __global__ __launch_bounds__(kWave)
                     if constexpr (kBias && E == 2) dl[rt] = join_left<T>(df[rt], ds[0][rt], ds[1][rt]);
                 }
                 if constexpr (kBias) {
-#pragma unroll 1
-                    for (int x = 0; x < a.axes; ++x) {
+#pragma unroll
+                    for (int x = 0; x < 3; ++x) {
+                        if (x >= a.axes) continue;
                         const int key = s_cell[x * kStep + (lane & (kStep - 1))];
                         uint32_t keys = static_cast<uint32_t>(__ballot((lane & (kStep - 1)) < left));
                         while (keys != 0) {
-                            const int k_low = least_of(key, keys);
+                            // The first key's cell in the middle of the window mostly does.
+                            int k_low = __builtin_amdgcn_readfirstlane(key) - 2 * kWindow;
+                            if (!__all(static_cast<uint32_t>(key - k_low) < 4 * kWindow)) k_low = least_of(key, keys);
                             keys &= ~static_cast<uint32_t>(__ballot(static_cast<uint32_t>(key - k_low) < 4 * kWindow));
                             const Vec8<T> ku = units<T>(s_cell + x * kStep, g, k_low + 4 * n);
                             f32x4 by_key[2 * kPairs];
@@ -285,20 +318,14 @@ __global__ __launch_bounds__(kWave)
                                 part[p] = join<T>(by_key[2 * p], by_key[2 * p + 1]);
                                 if constexpr (E == 2) part_left[p] = join_left<T>(part[p], by_key[2 * p], by_key[2 * p + 1]);
                             }
-                            uint64_t rows = ~uint64_t{0} >> (64 - min(here, RT * 16));
-                            const int query = s_query[x * kQueries + (lane & (kQueries - 1))];
-                            while (rows != 0) {
-                                int q_low = least_of(query, static_cast<uint32_t>(rows));
-                                if (kPairs == 2) {
-                                    const int other = s_query[x * kQueries + ((lane + 32) & (kQueries - 1))];
-                                    const int up = least_of(lane < 32 ? other : query, static_cast<uint32_t>(rows >> 32));
-                                    q_low = min(least_of(lane < 32 ? query : other, static_cast<uint32_t>(rows)), up);
-                                }
-                                rows &= ~__ballot(static_cast<uint32_t>(query - q_low) < 4 * kWindow);
+                            int q_low = q_least[x];
+                            while (true) {
                                 f32x4 sums = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                                 for (int p = 0; p < kPairs; ++p) {
-                                    const Vec8<T> qu = units<T>(s_query + x * kQueries + 32 * p, g, q_low + 4 * n);
+                                    const Vec8<T> qu = q_low == q_least[x]
+                                                           ? s_units[(x * kPairs + p) * kWave + lane]
+                                                           : units<T>(s_query + x * kQueries + 32 * p, g, q_low + 4 * n);
                                     sums = mma(qu, part[p], sums);
                                     if constexpr (E == 2) sums = mma(qu, part_left[p], sums);
                                 }
@@ -310,6 +337,11 @@ __global__ __launch_bounds__(kWave)
                                     to[r] += sums[r];
                                     wave_sync();
                                 }
+                                // On to the window that starts at the least cell after this one.
+                                q_low += 4 * kWindow;
+                                if (q_low > q_most[x]) break;
+                                const int q = s_query[x * kQueries + (lane & (kQueries - 1))];
+                                q_low = least_lane(q >= q_low ? q : INT32_MAX);
                             }
                         }
                     }
@@ -374,9 +406,12 @@ constexpr int key_tiles(int DP) { return sizeof(T) == 4 && DP == 128 ? 1 : 2; }
 // that chose it, for every head that shares the key head, 32 at a time.  With
 // blocks of whole steps (kWhole) a step's rows are neighbours in one row block;
 // otherwise the blocks' rows are strung together and each lane finds its own.
-template <typename T, int DP, bool kBias, bool kWhole>
-__global__ __launch_bounds__(kWave) __attribute__((amdgpu_waves_per_eu(DP * sizeof(T) <= 128 ? 2 : 1))) void attend_dkv_kernel(
-    AttendArgs a, AttendGrads gr, int tiles, int64_t items) {
+// W waves take every W-th step, and their sums are added in order.
+template <typename T, int DP, int W, bool kBias, bool kWhole>
+__global__ __launch_bounds__(kWave* W)
+    __attribute__((amdgpu_waves_per_eu(DP * sizeof(T) <= 128 ? 2 : 1))) void attend_dkv_kernel(AttendArgs a,
+                                                                                              AttendGrads gr, int tiles,
+                                                                                              int64_t items) {
     constexpr int DS = DP / 32, DT = DP / 16, KT = key_tiles<T>(DP), RT = kStep / 16, E = sizeof(T);
     constexpr int LD = turned_stride<T>(DP);
     extern __shared__ float4 s_raw[];
@@ -385,27 +420,30 @@ __global__ __launch_bounds__(kWave) __attribute__((amdgpu_waves_per_eu(DP * size
     if (item >= items) return;
     const int c = static_cast<int>(item % a.kv_heads);
     const int tile = static_cast<int>(item / a.kv_heads % tiles);
-    const int64_t block = item / a.kv_heads / tiles;
+    const int block = static_cast<int>(item / a.kv_heads / tiles);
+    const int wave = W == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const Rows kr = block_rows(a.k_starts, block, a.k_block, a.k_total);
     const int base = tile * KT * 16, left = kr.count - base;
     if (left <= 0) return;
 
-    T* s_q = reinterpret_cast<T*>(s_raw);
+    constexpr int kStage = 2 * kStep * LD * E + 6 * kStep * 4;  // bytes of a wave
+    T* s_q = reinterpret_cast<T*>(reinterpret_cast<char*>(s_raw) + wave * kStage);
     T* s_g = s_q + kStep * LD;
     int* s_cell = reinterpret_cast<int*>(s_g + kStep * LD);  // (3, 32)
     int* s_head = s_cell + 3 * kStep;                        // byte offset of the row's head's table
     float* s_lse = reinterpret_cast<float*>(s_head + kStep);
     float* s_delta = s_lse + kStep;
-    float* s_bias = s_delta + kStep;
+    float* s_bias = reinterpret_cast<float*>(reinterpret_cast<char*>(s_raw) + W * kStage);
     const int span = 2 * a.reach + 1, entries = a.axes * span, reach = 4 * a.reach;
     if constexpr (kBias) {
         const T* table = static_cast<const T*>(a.table);
-        for (int i = lane; i < a.share * entries; i += kWave) {
+        for (int i = threadIdx.x; i < a.share * entries; i += kWave * W) {
             const int hs = i / entries, e = i - hs * entries, axis = e / span;
             const int b = min(max(a.map[e - axis * span], 0), a.buckets - 1);
             s_bias[i] = static_cast<float>(table[(axis * a.buckets + b) * a.heads + c * a.share + hs]) * kLog2e;
         }
     }
+    if (W > 1 && kBias) __syncthreads();
     Vec8<T> kf[KT][DS], vf[KT][DS];
     int kc[KT][3];
     {
@@ -425,6 +463,20 @@ __global__ __launch_bounds__(kWave) __attribute__((amdgpu_waves_per_eu(DP * size
 #pragma unroll
                 for (int x = 0; x < 3; ++x) kc[kt][x] = x < a.axes ? cell_bytes(a.k_cells[at * a.axes + x]) : 0;
             }
+        }
+    }
+    int k_least[3] = {}, k_most[3] = {};
+    if constexpr (kBias) {
+#pragma unroll
+        for (int x = 0; x < 3; ++x) {
+            int lo = kc[0][x], hi = kc[0][x];
+#pragma unroll
+            for (int kt = 1; kt < KT; ++kt) {
+                lo = min(lo, kc[kt][x]);
+                hi = max(hi, kc[kt][x]);
+            }
+            k_least[x] = least_lane(lo);
+            k_most[x] = largest_lane(hi);
         }
     }
     f32x4 dk[KT][DT], dv[KT][DT];
@@ -521,8 +573,8 @@ __global__ __launch_bounds__(kWave) __attribute__((amdgpu_waves_per_eu(DP * size
                 }
             }
         };
-        load(0);
-        for (int step = 0; step < steps; ++step) {
+        if (wave < steps) load(wave);
+        for (int step = wave; step < steps; step += W) {
             wave_sync();
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt)
@@ -554,7 +606,17 @@ __global__ __launch_bounds__(kWave) __attribute__((amdgpu_waves_per_eu(DP * size
                         ds[rt][kt] = mma(gf[rt][s], vf[kt][s], ds[rt][kt]);
                     }
                 }
-            if (step + 1 < steps) load(step + 1);
+            // Whether no distance of the step is clamped.
+            bool close[3] = {};
+            if constexpr (kBias) {
+#pragma unroll
+                for (int x = 0; x < 3; ++x) {
+                    if (x >= a.axes) continue;
+                    const int mine = s_cell[x * kStep + (lane & (kStep - 1))];
+                    close[x] = __all(mine - k_least[x] <= reach && k_most[x] - mine <= reach);
+                }
+            }
+            if (step + W < steps) load(step + W);
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
                 const f32x4 l = *reinterpret_cast<const f32x4*>(s_lse + 16 * rt + 4 * g);
@@ -572,12 +634,22 @@ __global__ __launch_bounds__(kWave) __attribute__((amdgpu_waves_per_eu(DP * size
                         const int4 qc = *reinterpret_cast<const int4*>(s_cell + x * kStep + 16 * rt + 4 * g);
                         const int q[4] = {qc.x, qc.y, qc.z, qc.w};
                         const char* table = reinterpret_cast<const char*>(s_bias + x * span + a.reach);
+                        if (close[x]) {
 #pragma unroll
-                        for (int kt = 0; kt < KT; ++kt)
+                            for (int r = 0; r < 4; ++r) {
+                                const int from = q[r] + heads[r];
 #pragma unroll
-                            for (int r = 0; r < 4; ++r)
-                                p[rt][kt][r] += *reinterpret_cast<const float*>(
-                                    table + heads[r] + cell_distance(q[r], kc[kt][x], reach));
+                                for (int kt = 0; kt < KT; ++kt)
+                                    p[rt][kt][r] += *reinterpret_cast<const float*>(table + (from - kc[kt][x]));
+                            }
+                        } else {
+#pragma unroll
+                            for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                                for (int r = 0; r < 4; ++r)
+                                    p[rt][kt][r] += *reinterpret_cast<const float*>(
+                                        table + heads[r] + cell_distance(q[r], kc[kt][x], reach));
+                        }
                     }
                 }
 #pragma unroll
@@ -597,6 +669,29 @@ __global__ __launch_bounds__(kWave) __attribute__((amdgpu_waves_per_eu(DP * size
                     dk[kt][t] = mma(load_turned<T, LD>(s_q, t, n, g), df, dk[kt][t]);
                 }
             }
+        }
+    }
+    if constexpr (W > 1) {
+        constexpr int kPer = KT * DT * 8 * kWave;
+        float* s_part = reinterpret_cast<float*>(s_raw);
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < KT * DT; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                s_part[wave * kPer + (i * 8 + r) * kWave + lane] = dk[i / DT][i % DT][r];
+                s_part[wave * kPer + (i * 8 + 4 + r) * kWave + lane] = dv[i / DT][i % DT][r];
+            }
+        __syncthreads();
+        if (wave != 0) return;
+        for (int w = 1; w < W; ++w) {
+#pragma unroll
+            for (int i = 0; i < KT * DT; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    dk[i / DT][i % DT][r] += s_part[w * kPer + (i * 8 + r) * kWave + lane];
+                    dv[i / DT][i % DT][r] += s_part[w * kPer + (i * 8 + 4 + r) * kWave + lane];
+                }
         }
     }
 #pragma unroll
@@ -671,8 +766,10 @@ hipError_t launch_dq(const AttendArgs& a, const AttendGrads& g, hipStream_t stre
     const int64_t items = (kBias ? g.parts : static_cast<int64_t>(a.groups) * tiles) * a.heads;
     const int entries = a.axes * (2 * a.reach + 1);
     const size_t lds = kStep * turned_stride<T>(DP) * sizeof(T) + 3 * (kStep + 32 * ((RT + 1) / 2)) * sizeof(int) +
-                       (kBias ? entries + static_cast<size_t>(a.axes) * 4 * (2 * (a.reach + 2 * kWindow) - 1) : 0) *
-                           sizeof(float);
+                       (kBias ? (entries + static_cast<size_t>(a.axes) * 4 * (2 * (a.reach + 2 * kWindow) - 1)) *
+                                        sizeof(float) +
+                                    3 * ((RT + 1) / 2) * kWave * 8 * sizeof(T)
+                              : 0);
     const auto kernel = attend_dq_kernel<T, DP, RT, kBias>;
     const hipError_t e = allow_lds(kernel, lds);
     if (e != hipSuccess) return e;
@@ -680,25 +777,34 @@ hipError_t launch_dq(const AttendArgs& a, const AttendGrads& g, hipStream_t stre
     return hipGetLastError();
 }
 
-template <typename T, int DP, bool kBias, bool kWhole>
-hipError_t launch_dkv(const AttendArgs& a, const AttendGrads& g, hipStream_t stream) {
+template <typename T, int DP, int W, bool kBias, bool kWhole>
+hipError_t launch_dkv_waves(const AttendArgs& a, const AttendGrads& g, hipStream_t stream) {
     constexpr int kKeys = 16 * key_tiles<T>(DP);
     const int tiles = (a.k_block + kKeys - 1) / kKeys;
     const int64_t items = static_cast<int64_t>(a.blocks) * tiles * a.kv_heads;
-    const size_t lds = 2 * kStep * turned_stride<T>(DP) * sizeof(T) + 6 * kStep * sizeof(float) +
-                       (kBias ? static_cast<size_t>(a.share) * a.axes * (2 * a.reach + 1) * sizeof(float) : 0);
-    const auto kernel = attend_dkv_kernel<T, DP, kBias, kWhole>;
+    const size_t stage = W * (2 * kStep * turned_stride<T>(DP) * sizeof(T) + 6 * kStep * sizeof(float)) +
+                         (kBias ? static_cast<size_t>(a.share) * a.axes * (2 * a.reach + 1) * sizeof(float) : 0);
+    const size_t parts = W > 1 ? static_cast<size_t>(W) * key_tiles<T>(DP) * (DP / 16) * 8 * kWave * sizeof(float) : 0;
+    const size_t lds = std::max(stage, parts);
+    const auto kernel = attend_dkv_kernel<T, DP, W, kBias, kWhole>;
     const hipError_t e = allow_lds(kernel, lds);
     if (e != hipSuccess) return e;
-    kernel<<<static_cast<unsigned>(xcd_grid(items)), kWave, lds, stream>>>(a, g, tiles, items);
+    kernel<<<static_cast<unsigned>(xcd_grid(items)), kWave * W, lds, stream>>>(a, g, tiles, items);
     return hipGetLastError();
+}
+
+// Waves of a key tile: one where the tiles alone cover the chip several times.
+template <typename T, int DP, bool kBias, bool kWhole>
+hipError_t launch_dkv(const AttendArgs& a, const AttendGrads& g, hipStream_t stream) {
+    const int64_t waves = static_cast<int64_t>(a.blocks) * ((a.k_block + 31) / 32) * a.kv_heads;
+    return waves <= kSplitWaves ? launch_dkv_waves<T, DP, 4, kBias, kWhole>(a, g, stream)
+                                : launch_dkv_waves<T, DP, 1, kBias, kWhole>(a, g, stream);
 }
 
 template <typename T, int DP, bool kBias>
 hipError_t launch_pair(const AttendArgs& a, const AttendGrads& g, hipStream_t stream) {
-    constexpr int kWide = sizeof(T) == 2 && DP <= 32 ? 4 : 2;
-    hipError_t e = a.q_block <= 16 ? launch_dq<T, DP, 1, kBias>(a, g, stream)
-                                   : launch_dq<T, DP, kWide, kBias>(a, g, stream);
+    hipError_t e = a.q_block <= 16 ? launch_dq<T, DP, query_tiles(sizeof(T), DP, 16), kBias>(a, g, stream)
+                                   : launch_dq<T, DP, query_tiles(sizeof(T), DP, 17), kBias>(a, g, stream);
     if (e != hipSuccess) return e;
     if constexpr (kBias) {
         const int bins = a.axes * a.buckets;
@@ -721,10 +827,12 @@ hipError_t launch_type(const AttendArgs& a, const AttendGrads& g, hipStream_t st
 
 }  // namespace
 
-int attend_table_parts(int groups, int q_block, int heads) {
-    (void)q_block;
-    (void)heads;
-    return std::max(1, std::min(groups, kTableParts));
+int attend_table_parts(const AttendArgs& a, bool bf16) {
+    const int rows = 16 * query_tiles(bf16 ? 2 : 4, a.D <= 32 ? 32 : a.D <= 64 ? 64 : 128, a.q_block);
+    const int64_t tiles = static_cast<int64_t>(a.groups) * ((a.q_block + rows - 1) / rows);
+    const int64_t most = std::max(1, kTableWaves / a.heads);
+    const int64_t each = std::max<int64_t>(1, (tiles + most - 1) / most);  // tiles of a wave
+    return static_cast<int>(std::max<int64_t>(1, (tiles + each - 1) / each));
 }
 
 hipError_t launch_attend_backward(const AttendArgs& a, const AttendGrads& g, bool bf16, hipStream_t stream) {

@@ -1652,7 +1652,7 @@ struct AttendLayout {
     int64_t entries = 0;
     int parts = 0;
 };
-AttendLayout make_attend_layout(const AttendArgs& a) {
+AttendLayout make_attend_layout(const AttendArgs& a, bool bf16) {
     AttendLayout l;
     l.entries = static_cast<int64_t>(a.groups) * a.count;
     if (l.entries > 0) l.sort = make_layout(1, l.entries, 3, false);
@@ -1660,7 +1660,7 @@ AttendLayout make_attend_layout(const AttendArgs& a) {
     l.order = at; at = align_up(at + static_cast<size_t>(l.entries) * 8);
     l.runs = at; at = align_up(at + (static_cast<size_t>(a.blocks) + 1) * 4);
     l.delta = at; at = align_up(at + static_cast<size_t>(a.q_total) * a.heads * 4);
-    l.parts = attend_table_parts(a.groups, a.q_block, a.heads);
+    l.parts = attend_table_parts(a, bf16);
     l.table = at;
     if (a.table) at = align_up(at + static_cast<size_t>(l.parts) * a.heads * a.axes * a.buckets * 4);
     l.total = at;
@@ -1739,7 +1739,7 @@ int tbvh_attend_backward_workspace_size(const tbvh_attend_args* args, size_t* by
     if (!bytes) return fail(TBVH_ERR_INVALID_ARGUMENT, "%s: bytes is null", op);
     AttendArgs a;
     if (int r = check_attend(op, args, a)) return r;
-    *bytes = make_attend_layout(a).total;
+    *bytes = make_attend_layout(a, args->bf16 != 0).total;
     return ok();
 }
 
@@ -1757,7 +1757,7 @@ int tbvh_attend_backward(const tbvh_attend_args* args, const void* grad, void* d
     if (!multiple_of_16(grad) || !multiple_of_16(dq) || !multiple_of_16(dk) || !multiple_of_16(dv)) {
         return fail(TBVH_ERR_INVALID_ARGUMENT, "%s: gradients must be 16-byte aligned", op);
     }
-    const AttendLayout l = make_attend_layout(a);
+    const AttendLayout l = make_attend_layout(a, args->bf16 != 0);
     if (int r = check_workspace(op, ws, ws_bytes, l.total)) return r;
     const hipStream_t stream = static_cast<hipStream_t>(stream_ptr);
     SortBuffers sb = sort_buffers(ws, l.sort);
