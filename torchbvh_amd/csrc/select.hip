@@ -43,10 +43,71 @@ __device__ __forceinline__ float box_score(const float* __restrict__ box, const 
     return bad ? INFINITY : score;
 }
 
-// One wave per block of queries.  Lane i holds the i-th best key so far, a key
-// being (score, block) in 64 bits; 64 boxes are scored at a time and those
-// that beat the last kept key are put in their places one by one.
+// The boxes of every 64 consecutive blocks, whatever their clouds: one wave each.
+// A block's score is never below its 64's: subtraction, maximum, square and sum
+// all round monotonically.
 template <int D>
+__global__ __launch_bounds__(kWave) void coarse_kernel(const float* __restrict__ boxes, int blocks,
+                                                       float* __restrict__ coarse) {
+    const int b = blockIdx.x * kWave + lane_id();
+#pragma unroll
+    for (int x = 0; x < 2 * D; ++x) {
+        float v = x < D ? INFINITY : -INFINITY;
+        if (b < blocks) v = x < D ? fminf(v, boxes[b * int64_t{2 * D} + x]) : fmaxf(v, boxes[b * int64_t{2 * D} + x]);
+        v = x < D ? wave_min(v) : wave_max(v);
+        if (lane_id() == 0) coarse[blockIdx.x * 2 * D + x] = v;
+    }
+}
+
+// Lanes in ascending order of their keys, and of two ascending lists the 64 least
+// (bitonic networks over the wave).
+__device__ __forceinline__ uint64_t keep(uint64_t a, uint64_t b, bool least) { return (a < b) == least ? a : b; }
+__device__ __forceinline__ uint64_t finish(uint64_t key) {
+#pragma unroll
+    for (int j = kWave / 2; j > 0; j >>= 1) key = keep(key, shfl64(key, lane_id() ^ j), (lane_id() & j) == 0);
+    return key;
+}
+__device__ __forceinline__ uint64_t sorted(uint64_t key) {
+#pragma unroll
+    for (int k = 2; k < kWave; k <<= 1) {
+#pragma unroll
+        for (int j = k >> 1; j > 0; j >>= 1)
+            key = keep(key, shfl64(key, lane_id() ^ j), ((lane_id() & j) == 0) == ((lane_id() & k) == 0));
+    }
+    return finish(key);
+}
+__device__ __forceinline__ uint64_t merged(uint64_t a, uint64_t b) {
+    return finish(keep(a, shfl64(b, kWave - 1 - lane_id()), true));
+}
+
+// The 64 least keys so far, lane i the i-th, and the largest that still counts.
+struct Best {
+    uint64_t key = kNoBlock, limit = kNoBlock;
+    __device__ __forceinline__ void take(uint64_t x, int count) {
+        uint64_t todo = __ballot(x < limit);
+        // From about ten keys on the networks are shorter than putting each in its
+        // place (27 exchanges against three a key).
+        if (__popcll(todo) > 10) {
+            key = key_empty() ? sorted(x) : merged(key, sorted(x));
+            limit = shfl64(key, count - 1);
+            return;
+        }
+        for (; todo != 0; todo &= todo - 1) {
+            const uint64_t one = shfl64(x, __builtin_ctzll(todo));
+            if (one >= limit) continue;
+            const int at = __popcll(__ballot(key < one));
+            const uint64_t up = shfl64(key, lane_id() > 0 ? lane_id() - 1 : 0);
+            key = lane_id() < at ? key : lane_id() == at ? one : up;
+            limit = shfl64(key, count - 1);
+        }
+    }
+    __device__ __forceinline__ bool key_empty() const { return __ballot(key != kNoBlock) == 0; }
+};
+
+// One wave per block of queries.  With kCoarse it scores the boxes of 64 blocks
+// first, takes the nearest of them, and then only those that can still hold one of
+// the `count` least.
+template <int D, bool kCoarse>
 __global__ __launch_bounds__(kWave) void select_kernel(SelectArgs a) {
     const int lane = lane_id();
     const int64_t group = blockIdx.x;
@@ -71,33 +132,72 @@ __global__ __launch_bounds__(kWave) void select_kernel(SelectArgs a) {
     const int cloud = cloud_of(a.q_clouds, a.clouds, group);
     const int64_t first = cloud < 0 ? 0 : max(a.k_clouds[cloud], int64_t{0});
     const int64_t last = cloud < 0 ? 0 : min(a.k_clouds[cloud + 1], static_cast<int64_t>(a.blocks));
-    uint64_t best = kNoBlock, limit = kNoBlock;
-    for (int64_t b0 = first; b0 < last; b0 += kWave) {
+    Best best;
+    const auto visit = [&](int64_t b0) {
         const int64_t b = b0 + lane;
         uint64_t key = kNoBlock;
-        if (b < last) {
+        if (b >= first && b < last) {
             const float score = box_score<D>(a.boxes + b * 2 * D, centre);
             if (score < INFINITY) key = static_cast<uint64_t>(__float_as_uint(score)) << 32 | static_cast<uint32_t>(b);
         }
-        for (uint64_t todo = __ballot(key < limit); todo != 0; todo &= todo - 1) {
-            const uint64_t x = shfl64(key, __builtin_ctzll(todo));
-            if (x >= limit) continue;
-            const int at = __popcll(__ballot(best < x));
-            const uint64_t up = shfl64(best, lane > 0 ? lane - 1 : 0);
-            best = lane < at ? best : lane == at ? x : up;
-            limit = shfl64(best, a.count - 1);
+        best.take(key, a.count);
+    };
+    if constexpr (!kCoarse) {
+        for (int64_t b = first; b < last; b += kWave) visit(b);
+    } else if (first < last) {
+        const int64_t begin = first / kWave, end = (last + kWave - 1) / kWave;
+        // A set's key is below the key of each block in it.
+        const auto bound = [&](int64_t set) {
+            uint64_t key = kNoBlock;
+            if (set < end) {
+                const float score = box_score<D>(a.coarse + set * 2 * D, centre);
+                if (score < INFINITY)
+                    key = static_cast<uint64_t>(__float_as_uint(score)) << 32 | static_cast<uint32_t>(set * kWave);
+            }
+            return key;
+        };
+        uint64_t nearest = kNoBlock;
+        for (int64_t s = begin; s < end; s += kWave) nearest = keep(nearest, bound(s + lane), true);
+#pragma unroll
+        for (int j = 1; j < kWave; j <<= 1) nearest = keep(nearest, shfl64(nearest, lane ^ j), true);
+        if (nearest != kNoBlock) {
+            const int64_t chosen = static_cast<uint32_t>(nearest) / kWave;
+            visit(chosen * kWave);
+            for (int64_t s = begin; s < end; s += kWave) {
+                const uint64_t key = bound(s + lane);
+                for (uint64_t todo = __ballot(key < best.limit && s + lane != chosen); todo != 0;) {
+                    const int at = __builtin_ctzll(todo);
+                    visit((s + at) * kWave);
+                    todo &= todo - 1;
+                    todo &= __ballot(key < best.limit);
+                }
+            }
         }
     }
-    if (lane < a.count) a.out[group * a.count + lane] = best == kNoBlock ? -1 : static_cast<int32_t>(best);
+    if (lane < a.count) a.out[group * a.count + lane] = best.key == kNoBlock ? -1 : static_cast<int32_t>(best.key);
 }
 
 }  // namespace
 
+namespace {
+// From this many blocks on the extra launch and level pay.
+constexpr int kCoarseBlocks = 512;
+
+template <int D>
+hipError_t launch(const SelectArgs& a, hipStream_t stream) {
+    if (a.blocks >= kCoarseBlocks) {
+        coarse_kernel<D><<<(a.blocks + kWave - 1) / kWave, kWave, 0, stream>>>(a.boxes, a.blocks, a.coarse);
+        select_kernel<D, true><<<a.groups, kWave, 0, stream>>>(a);
+    } else {
+        select_kernel<D, false><<<a.groups, kWave, 0, stream>>>(a);
+    }
+    return hipGetLastError();
+}
+}  // namespace
+
 hipError_t launch_select(const SelectArgs& a, int D, hipStream_t stream) {
     if (a.groups == 0) return hipSuccess;
-    if (D == 2) select_kernel<2><<<a.groups, kWave, 0, stream>>>(a);
-    else select_kernel<3><<<a.groups, kWave, 0, stream>>>(a);
-    return hipGetLastError();
+    return D == 2 ? launch<2>(a, stream) : launch<3>(a, stream);
 }
 
 }  // namespace tbvh
