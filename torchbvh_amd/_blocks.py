@@ -59,11 +59,9 @@ class RelativeBias(NamedTuple):
     key_cells: torch.Tensor    # (key rows, axes) int32
 
 
-def _refuse(op: str, *rules) -> None:
-    """ValueError for the first rule (holds, message) that does not hold."""
-    for holds, message in rules:
-        if not holds:
-            raise ValueError(f"{op}: {message}")
+def _require(op: str, holds: bool, message: str) -> None:
+    if not holds:
+        raise ValueError(f"{op}: {message}")
 
 
 def block_layout(source, block_size: int = 64, *, device=None) -> BlockLayout:
@@ -71,7 +69,7 @@ def block_layout(source, block_size: int = 64, *, device=None) -> BlockLayout:
     clouds given as ``(B + 1,)`` int64 CUDA offsets (read back to the host
     once)."""
     op = "block_layout"
-    _refuse(op, (isinstance(block_size, int) and 1 <= block_size <= MAX_BLOCK, f"block_size must be 1 to {MAX_BLOCK}"))
+    _require(op, isinstance(block_size, int) and 1 <= block_size <= MAX_BLOCK, f"block_size must be 1 to {MAX_BLOCK}")
     if isinstance(source, RaggedBVHHandle):
         source = live_payload(source, RaggedBVHHandle, op)["batch_offsets"]
     elif isinstance(source, (BVHHandle, BatchedBVHHandle)):
@@ -84,9 +82,9 @@ def block_layout(source, block_size: int = 64, *, device=None) -> BlockLayout:
         total = int(source[-1]) if source.dim() == 1 and source.numel() and source.dtype == torch.int64 else 0
         offsets = check_offsets(op, source, total_rows=total, device=device)
     else:
-        _refuse(op, (isinstance(source, tuple) and len(source) == 2, "source must be a handle, (B, N) or offsets"))
+        _require(op, isinstance(source, tuple) and len(source) == 2, "source must be a handle, (B, N) or offsets")
         B, N = (int(x) for x in source)
-        _refuse(op, (B >= 1 and N >= 0, "need B >= 1 and N >= 0"))
+        _require(op, B >= 1 and N >= 0, "need B >= 1 and N >= 0")
         offsets = list(range(0, B * N + 1, N)) if N else [0] * (B + 1)
     device = torch.device("cuda") if device is None else torch.device(device)
     bounds = torch.tensor(offsets, dtype=torch.int64)
@@ -102,8 +100,8 @@ def block_boxes(bvh: AnyHandle, block_size: int = 64) -> torch.Tensor:
     that `block_layout` makes of a handle with the same ``block_size``, a power
     of two: the tree's nodes over so many leaves."""
     op = "block_boxes"
-    _refuse(op, (isinstance(block_size, int) and 1 <= block_size <= MAX_BLOCK and block_size & (block_size - 1) == 0,
-                 f"block_size must be a power of two up to {MAX_BLOCK}"))
+    _require(op, isinstance(block_size, int) and 1 <= block_size <= MAX_BLOCK and block_size & (block_size - 1) == 0,
+             f"block_size must be a power of two up to {MAX_BLOCK}")
     if isinstance(bvh, RaggedBVHHandle):
         live_payload(bvh, RaggedBVHHandle, op)
         return torch.cat([block_boxes(h, block_size) for h in bvh._handles])
@@ -126,7 +124,7 @@ def relative_buckets(sizes: int, max_distance: int, *, device=None) -> torch.Ten
     positive and ``sizes .. 2 sizes - 2`` negative distances, so a table needs
     ``2 sizes - 1`` buckets."""
     op = "relative_buckets"
-    _refuse(op, (sizes >= 2 and max_distance >= 1, "need sizes >= 2 and max_distance >= 1"))
+    _require(op, sizes >= 2 and max_distance >= 1, "need sizes >= 2 and max_distance >= 1")
     near = max(sizes // 2, 1)
 
     def size(d: int) -> int:
@@ -141,12 +139,15 @@ def relative_buckets(sizes: int, max_distance: int, *, device=None) -> torch.Ten
 
 
 def _check_layout(op: str, layout: BlockLayout, name: str, device: torch.device) -> None:
-    ok = isinstance(layout, BlockLayout) and all(
-        isinstance(t, torch.Tensor) and t.dtype == torch.int64 and t.dim() == 1 and t.numel() >= 1 and t.is_contiguous()
-        for t in layout[:3])
-    _refuse(op, (ok and layout.offsets.numel() == layout.clouds.numel() >= 2 and 1 <= layout.block_size <= MAX_BLOCK,
-                 f"{name} must be a BlockLayout (see block_layout)"),
-            (ok and all(t.device == device for t in layout[:3]), f"{name} must be on the same device as the rows"))
+    ok = isinstance(layout, BlockLayout) and 1 <= layout.block_size <= MAX_BLOCK
+    if ok:
+        for t in layout[:3]:
+            ok = ok and (isinstance(t, torch.Tensor) and t.dtype == torch.int64 and t.dim() == 1 and t.numel() >= 1
+                         and t.is_contiguous())
+    if not (ok and layout.offsets.numel() == layout.clouds.numel() >= 2):
+        raise ValueError(f"{op}: {name} must be a BlockLayout (see block_layout)")
+    if not layout.offsets.device == layout.starts.device == layout.clouds.device == device:
+        raise ValueError(f"{op}: {name} must be on the same device as the rows")
 
 
 def select_blocks(queries: torch.Tensor, boxes: torch.Tensor, count: int, query_layout: BlockLayout,
@@ -161,19 +162,26 @@ def select_blocks(queries: torch.Tensor, boxes: torch.Tensor, count: int, query_
     Coordinates that are NaN are left out of a block's box; blocks at no finite
     distance are not chosen."""
     op = "select_blocks"
-    _refuse(op, (queries.dim() == 2, "queries must have shape (T, D)"),
-            (queries.dim() == 2 and queries.size(1) in SUPPORTED_DIMS, "D must be 2 or 3"))
+    if queries.dim() != 2:
+        raise ValueError(f"{op}: queries must have shape (T, D)")
+    if queries.size(1) not in SUPPORTED_DIMS:
+        raise ValueError(f"{op}: D must be 2 or 3")
     check_cuda_f32(op, queries, "queries")
     check_cuda_f32(op, boxes, "boxes")
     _check_layout(op, query_layout, "query_layout", queries.device)
     _check_layout(op, key_layout, "key_layout", queries.device)
-    _refuse(op, (boxes.dim() == 2 and boxes.size(1) == 2 * queries.size(1), "boxes must have shape (blocks, 2 D)"),
-            (boxes.device == queries.device, "boxes must be on the same device as queries"),
-            (boxes.size(0) == key_layout.starts.numel() - 1, "boxes must have a row for every block of key_layout"),
-            (query_layout.clouds.numel() == key_layout.clouds.numel(), "the layouts must have the same clouds"),
-            (1 <= count <= MAX_SELECTED, f"count must be 1 to {MAX_SELECTED}"))
-    return _C.select_blocks(dense(queries.detach()), query_layout.starts, query_layout.clouds, query_layout.block_size,
-                            dense(boxes.detach()), key_layout.clouds, int(count))
+    if boxes.dim() != 2 or boxes.size(1) != 2 * queries.size(1):
+        raise ValueError(f"{op}: boxes must have shape (blocks, 2 D)")
+    if boxes.device != queries.device:
+        raise ValueError(f"{op}: boxes must be on the same device as queries")
+    if boxes.size(0) != key_layout.starts.numel() - 1:
+        raise ValueError(f"{op}: boxes must have a row for every block of key_layout")
+    if query_layout.clouds.numel() != key_layout.clouds.numel():
+        raise ValueError(f"{op}: the layouts must have the same clouds")
+    if not 1 <= count <= MAX_SELECTED:
+        raise ValueError(f"{op}: count must be 1 to {MAX_SELECTED}")
+    return _C.select_blocks(dense(queries), query_layout.starts, query_layout.clouds, query_layout.block_size,
+                            dense(boxes), key_layout.clouds, int(count))
 
 
 def _rows_of(t: torch.Tensor) -> torch.Tensor:
@@ -230,42 +238,67 @@ def block_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, selected:
     nothing, a block chosen twice counts twice, and rows for which nothing is
     chosen are zero."""
     op = "block_attention"
-    _refuse(op, *((t.dim() == 3, f"{n} must have shape (rows, heads, D)") for n, t in (("q", q), ("k", k), ("v", v))))
-    _refuse(op, (q.is_cuda, "q must be a CUDA tensor"), (q.dtype in _TYPES, "q must be float32 or bfloat16"),
-            (k.dtype == q.dtype and v.dtype == q.dtype, "k and v must have q's type"),
-            (k.device == q.device and v.device == q.device, "k and v must be on the same device as q"),
-            (k.shape == v.shape, "k and v must have the same shape"),
-            (1 <= q.size(2) <= MAX_CHANNELS, f"D must be 1 to {MAX_CHANNELS}"),
-            (k.size(2) == q.size(2), "k and v must have q's channels"),
-            (k.size(1) >= 1 and q.size(1) >= 1 and q.size(1) % k.size(1) == 0,
-             "q's heads must be a multiple of k's"))
-    _check_layout(op, query_layout, "query_layout", q.device)
-    _check_layout(op, key_layout, "key_layout", q.device)
-    _refuse(op, (isinstance(selected, torch.Tensor) and selected.dim() == 2
-                 and selected.size(0) == query_layout.starts.numel() - 1,
-                 "selected must have shape (blocks of query_layout, count)"),
-            (selected.dtype == torch.int32, "selected must be int32"),
-            (selected.device == q.device, "selected must be on the same device as q"))
+    if not q.dim() == k.dim() == v.dim() == 3:
+        name = "q" if q.dim() != 3 else "k" if k.dim() != 3 else "v"
+        raise ValueError(f"{op}: {name} must have shape (rows, heads, D)")
+    device, heads, D = q.device, q.size(1), q.size(2)
+    if not q.is_cuda:
+        raise ValueError(f"{op}: q must be a CUDA tensor")
+    if q.dtype not in _TYPES:
+        raise ValueError(f"{op}: q must be float32 or bfloat16")
+    if not q.dtype == k.dtype == v.dtype:
+        raise ValueError(f"{op}: k and v must have q's type")
+    if not device == k.device == v.device:
+        raise ValueError(f"{op}: k and v must be on the same device as q")
+    if k.shape != v.shape:
+        raise ValueError(f"{op}: k and v must have the same shape")
+    if not 1 <= D <= MAX_CHANNELS:
+        raise ValueError(f"{op}: D must be 1 to {MAX_CHANNELS}")
+    if k.size(2) != D:
+        raise ValueError(f"{op}: k and v must have q's channels")
+    if k.size(1) < 1 or heads < 1 or heads % k.size(1) != 0:
+        raise ValueError(f"{op}: q's heads must be a multiple of k's")
+    _check_layout(op, query_layout, "query_layout", device)
+    _check_layout(op, key_layout, "key_layout", device)
+    if not isinstance(selected, torch.Tensor) or selected.dim() != 2 or selected.size(0) != query_layout.starts.numel() - 1:
+        raise ValueError(f"{op}: selected must have shape (blocks of query_layout, count)")
+    if selected.dtype != torch.int32:
+        raise ValueError(f"{op}: selected must be int32")
+    if selected.device != device:
+        raise ValueError(f"{op}: selected must be on the same device as q")
     table = places = None
     if bias is not None:
-        table, buckets, query_cells, key_cells = bias
-        _refuse(op, (table.dim() == 3 and 1 <= table.size(0) <= 3 and table.size(2) == q.size(1),
-                     "bias.table must have shape (axes, buckets, heads) with 1 to 3 axes and q's heads"),
-                (table.dtype == q.dtype, "bias.table must have q's type"),
-                (1 <= table.size(0) * table.size(1) <= 256, "bias.table must have at most 256 axes * buckets"),
-                (buckets.dim() == 1 and buckets.numel() % 2 == 1 and buckets.dtype == torch.int32,
-                 "bias.buckets must be int32 with an odd number of entries"),
-                (table.size(0) * buckets.numel() * (q.size(1) // k.size(1)) <= 4096,
-                 "bias.buckets must have at most 4096 / (axes * heads per key head) entries"),
-                *((t.dim() == 2 and tuple(t.shape) == (n, table.size(0)) and t.dtype == torch.int32,
-                   f"bias.{what} must be int32 of shape (rows, axes)")
-                  for what, t, n in (("query_cells", query_cells, q.size(0)), ("key_cells", key_cells, k.size(0)))),
-                *((t.device == q.device, "the bias must be on the same device as q")
-                  for t in (table, buckets, query_cells, key_cells)))
-        table, places = dense(table), tuple(dense(t.detach()) for t in (buckets, query_cells, key_cells))
-    D = q.size(2)
+        _check_bias(op, bias, q, k)
+        table, places = dense(bias.table), tuple(dense(t) for t in bias[1:])
     scale = D**-0.5 if scale is None else float(scale)
     if D % 8:
         q, k, v = (torch.nn.functional.pad(t, (0, -D % 8)) for t in (q, k, v))
-    out = _Attend.apply(q, k, v, table, dense(selected.detach()), query_layout, key_layout, scale, places)
+    selected = dense(selected)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
+                                    or (table is not None and table.requires_grad)):
+        out = _Attend.apply(q, k, v, table, selected, query_layout, key_layout, scale, places)
+    else:
+        out = _C.attend(_rows_of(q), _rows_of(k), _rows_of(v), selected, query_layout.starts, key_layout.starts,
+                        query_layout.block_size, key_layout.block_size, scale,
+                        None if table is None else (table, *places), False)[0]
     return out[..., :D] if D % 8 else out
+
+
+def _check_bias(op: str, bias: RelativeBias, q: torch.Tensor, k: torch.Tensor) -> None:
+    table, buckets, query_cells, key_cells = bias
+    axes = table.size(0) if table.dim() == 3 else 0
+    if not 1 <= axes <= 3 or table.size(2) != q.size(1):
+        raise ValueError(f"{op}: bias.table must have shape (axes, buckets, heads) with 1 to 3 axes and q's heads")
+    if table.dtype != q.dtype:
+        raise ValueError(f"{op}: bias.table must have q's type")
+    if not 1 <= axes * table.size(1) <= 256:
+        raise ValueError(f"{op}: bias.table must have at most 256 axes * buckets")
+    if buckets.dim() != 1 or buckets.numel() % 2 != 1 or buckets.dtype != torch.int32:
+        raise ValueError(f"{op}: bias.buckets must be int32 with an odd number of entries")
+    if axes * buckets.numel() * (q.size(1) // k.size(1)) > 4096:
+        raise ValueError(f"{op}: bias.buckets must have at most 4096 / (axes * heads per key head) entries")
+    for what, t, rows in (("query_cells", query_cells, q.size(0)), ("key_cells", key_cells, k.size(0))):
+        if t.dim() != 2 or t.size(0) != rows or t.size(1) != axes or t.dtype != torch.int32:
+            raise ValueError(f"{op}: bias.{what} must be int32 of shape (rows, axes)")
+    if not q.device == table.device == buckets.device == query_cells.device == key_cells.device:
+        raise ValueError(f"{op}: the bias must be on the same device as q")

@@ -255,6 +255,24 @@ def _address(t: torch.Tensor | None):
     return None if t is None else t.data_ptr()
 
 
+class _Here:
+    """`with torch.cuda.device(device)` for a device that is the current one."""
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_here = _Here()
+
+
+def _on(device: torch.device):
+    """Makes `device` the current one (a few microseconds unless it is already)."""
+    return _here if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
 def _stream(device: torch.device):
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
@@ -1253,8 +1271,8 @@ class _NativeOps:
         dev = queries.device
         out = torch.empty((groups, count), dtype=torch.int32, device=dev)
         L = load()
-        with torch.cuda.device(dev):
-            ws = _workspace(_size(L.tbvh_select_blocks_workspace_size, blocks, dim), dev)
+        with _on(dev):
+            ws = _workspace(_select_size(blocks, dim), dev)
             _check(L.tbvh_select_blocks(
                 _ptr(queries), queries.size(0), _ptr(q_starts), _ptr(q_clouds), groups, q_block, _ptr(boxes),
                 _ptr(k_clouds), blocks, q_clouds.numel() - 1, dim, count, _ptr(out), _ptr(ws), ws.numel(), _stream(dev)))
@@ -1271,7 +1289,7 @@ class _NativeOps:
         lse = torch.empty((q.size(1), q.size(0)), dtype=torch.float32, device=q.device) if want_lse else None
         rest = torch.empty_like(out) if want_lse and bias is not None and q.dtype == torch.bfloat16 else None
         args.out, args.lse, args.rest = out.data_ptr(), lse.data_ptr() if want_lse else None, _address(rest)
-        with torch.cuda.device(q.device):
+        with _on(q.device):
             _check(load().tbvh_attend(ctypes.byref(args), _stream(q.device)))
         return out, lse, rest
 
@@ -1287,7 +1305,7 @@ class _NativeOps:
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
         dtable = None if bias is None else torch.empty(bias[0].shape, dtype=q.dtype, device=dev)
         L = load()
-        with torch.cuda.device(dev):
+        with _on(dev):
             ws = _workspace(_size(L.tbvh_attend_backward_workspace_size, ctypes.byref(args)), dev)
             _check(L.tbvh_attend_backward(ctypes.byref(args), _ptr(grad), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dtable),
                                           _ptr(ws), ws.numel(), _stream(dev)))
@@ -1303,8 +1321,8 @@ class _NativeOps:
         y = torch.empty_like(x)
         mean, rstd = (torch.empty((clouds, groups), dtype=torch.float32, device=dev) for _ in range(2))
         L = load()
-        with torch.cuda.device(dev):
-            ws = _workspace(_size(L.tbvh_group_norm_workspace_size, rows, clouds, channels, groups), dev)
+        with _on(dev):
+            ws = _workspace(_norm_size(rows, clouds, channels, groups), dev)
             _check(L.tbvh_group_norm(_ptr(x), _ptr(offsets), rows, clouds, channels, groups, _ptr(weight), _ptr(bias),
                                      wide, x.dtype == torch.bfloat16, eps, activation, _ptr(y), _ptr(mean), _ptr(rstd),
                                      _ptr(ws), ws.numel(), _stream(dev)))
@@ -1324,13 +1342,23 @@ class _NativeOps:
         dweight = torch.empty_like(weight) if want_dweight else None
         dbias = torch.empty_like(bias) if want_dbias else None
         L = load()
-        with torch.cuda.device(dev):
-            ws = _workspace(_size(L.tbvh_group_norm_workspace_size, rows, clouds, channels, groups), dev)
+        with _on(dev):
+            ws = _workspace(_norm_size(rows, clouds, channels, groups), dev)
             _check(L.tbvh_group_norm_backward(
                 _ptr(x), _ptr(grad), _ptr(offsets), rows, clouds, channels, groups, _ptr(weight), _ptr(bias), wide,
                 x.dtype == torch.bfloat16, eps, activation, _ptr(mean), _ptr(rstd), _ptr(dx), _ptr(dweight),
                 _ptr(dbias), _ptr(ws), ws.numel(), _stream(dev)))
         return dx, dweight, dbias
+
+
+@functools.lru_cache(maxsize=256)
+def _select_size(blocks: int, dim: int) -> int:
+    return _size(load().tbvh_select_blocks_workspace_size, blocks, dim)
+
+
+@functools.lru_cache(maxsize=256)
+def _norm_size(rows: int, clouds: int, channels: int, groups: int) -> int:
+    return _size(load().tbvh_group_norm_workspace_size, rows, clouds, channels, groups)
 
 
 def _require_norm(op, x, offsets, weight, bias) -> bool:
@@ -1349,37 +1377,37 @@ def _require_norm(op, x, offsets, weight, bias) -> bool:
 
 
 def _attend_args(op, q, k, v, selected, q_starts, k_starts, q_block, k_block, scale, bias) -> AttendArgs:
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        _require(t.is_cuda and t.device == q.device and t.dim() == 3 and t.dtype == q.dtype
-                 and t.dtype in (torch.float32, torch.bfloat16) and (t.stride(2) == 1 or t.numel() == 0), op,
-                 f"{name} must be a CUDA tensor (rows, heads, D) with contiguous channels, float32 or bfloat16 like q")
-    _require(k.shape == v.shape and k.size(2) == q.size(2), op, "k and v must have one shape, and q's channels")
-    for name, t in (("q_starts", q_starts), ("k_starts", k_starts)):
-        _require_device_i64(op, t, name)
-        _require(t.device == q.device and t.dim() == 1 and t.numel() >= 1, op, f"{name} must be (blocks + 1,) beside q")
-    groups = int(q_starts.numel()) - 1
-    _require(selected.is_cuda and selected.device == q.device and selected.dtype == torch.int32
-             and selected.is_contiguous() and selected.dim() == 2 and selected.size(0) == groups, op,
-             "selected must be a contiguous CUDA int32 tensor (groups, count)")
+    device, kind = q.device, q.dtype
+    for t in (q, k, v):
+        if (t.device != device or t.dim() != 3 or t.dtype != kind or kind not in (torch.float32, torch.bfloat16)
+                or not (t.stride(2) == 1 or t.numel() == 0)):
+            raise RuntimeError(f"{op}: q, k and v must be CUDA tensors (rows, heads, D) with contiguous channels, "
+                               "float32 or bfloat16, on one device")
+    _require(q.is_cuda and k.shape == v.shape and k.size(2) == q.size(2), op, "k and v must have one shape, and q's channels")
+    for t in (q_starts, k_starts):
+        if t.device != device or t.dtype != torch.int64 or t.dim() != 1 or t.numel() < 1 or not t.is_contiguous():
+            raise RuntimeError(f"{op}: q_starts and k_starts must be contiguous int64 (blocks + 1,) beside q")
+    groups = q_starts.numel() - 1
+    if (selected.device != device or selected.dtype != torch.int32 or not selected.is_contiguous()
+            or selected.dim() != 2 or selected.size(0) != groups):
+        raise RuntimeError(f"{op}: selected must be a contiguous CUDA int32 tensor (groups, count)")
     args = AttendArgs(
-        q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), q_row_stride=q.stride(0), q_head_stride=q.stride(1),
-        k_row_stride=k.stride(0), k_head_stride=k.stride(1), v_row_stride=v.stride(0), v_head_stride=v.stride(1),
-        q_rows=q.size(0), k_rows=k.size(0), selected=selected.data_ptr(), q_starts=q_starts.data_ptr(),
-        k_starts=k_starts.data_ptr(), groups=groups, blocks=int(k_starts.numel()) - 1, count=selected.size(1),
-        q_block=q_block, k_block=k_block, heads=q.size(1), kv_heads=k.size(1), D=q.size(2),
-        bf16=q.dtype == torch.bfloat16, scale=scale)
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0),
+        v.stride(1), q.size(0), k.size(0), selected.data_ptr(), q_starts.data_ptr(), k_starts.data_ptr(), groups,
+        k_starts.numel() - 1, selected.size(1), q_block, k_block, q.size(1), k.size(1), q.size(2),
+        kind == torch.bfloat16, scale)
     if bias is not None:
         table, spread, q_cells, k_cells = bias
-        _require(table.is_contiguous() and table.dtype == q.dtype and table.dim() == 3 and table.size(2) == q.size(1)
-                 and table.device == q.device, op, "table must be a contiguous (axes, buckets, heads) tensor like q")
-        for name, t, shape in (("map", spread, None), ("q_cells", q_cells, (q.size(0), table.size(0))),
-                               ("k_cells", k_cells, (k.size(0), table.size(0)))):
-            _require(t.is_contiguous() and t.dtype == torch.int32 and t.device == q.device
-                     and (shape is None or tuple(t.shape) == shape), op, f"{name} must be a contiguous int32 tensor")
-        _require(spread.dim() == 1 and spread.numel() % 2 == 1, op, "map must hold an odd number of entries")
+        _require(table.is_contiguous() and table.dtype == kind and table.dim() == 3 and table.size(2) == q.size(1)
+                 and table.device == device, op, "table must be a contiguous (axes, buckets, heads) tensor like q")
+        for t, rows in ((spread, -1), (q_cells, q.size(0)), (k_cells, k.size(0))):
+            if (not t.is_contiguous() or t.dtype != torch.int32 or t.device != device
+                    or (t.dim() != 1 or t.numel() % 2 != 1 if rows < 0
+                        else t.dim() != 2 or t.size(0) != rows or t.size(1) != table.size(0))):
+                raise RuntimeError(f"{op}: map must be int32 with an odd number of entries, cells (rows, axes)")
         args.table, args.map = table.data_ptr(), spread.data_ptr()
         args.q_cells, args.k_cells = q_cells.data_ptr(), k_cells.data_ptr()
-        args.axes, args.buckets, args.reach = table.size(0), table.size(1), int(spread.numel()) // 2
+        args.axes, args.buckets, args.reach = table.size(0), table.size(1), spread.numel() // 2
     return args
 
 

@@ -7,7 +7,7 @@ from __future__ import annotations
 
 import torch
 
-from ._blocks import BlockLayout, _check_layout, _refuse
+from ._blocks import BlockLayout, _check_layout
 from ._native import _C
 from ._validation import dense
 
@@ -53,28 +53,43 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None
     ``layout``; float32 or bfloat16.  ``weight`` and ``bias (C,)`` are of its type or
     float32."""
     op = "group_norm_act"
-    _refuse(op, (x.dim() == 2 or (x.dim() == 3 and layout is None),
-                 "x must have shape (N, C) or (B, N, C), or (total_N, C) with a layout"),
-            (x.is_cuda, "x must be a CUDA tensor"),
-            (x.dtype in (torch.float32, torch.bfloat16), "x must be float32 or bfloat16"),
-            (num_groups >= 1 and x.size(-1) >= 1 and x.size(-1) % num_groups == 0,
-             "channels must be a multiple of num_groups"),
-            (activation in ACTIVATIONS, f"activation must be one of {', '.join(ACTIVATIONS)}"),
-            (eps >= 0.0, "eps must be >= 0"))
+    if x.dim() != 2 and (x.dim() != 3 or layout is not None):
+        raise ValueError(f"{op}: x must have shape (N, C) or (B, N, C), or (total_N, C) with a layout")
+    if not x.is_cuda:
+        raise ValueError(f"{op}: x must be a CUDA tensor")
+    if x.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError(f"{op}: x must be float32 or bfloat16")
+    if num_groups < 1 or x.size(-1) < 1 or x.size(-1) % num_groups != 0:
+        raise ValueError(f"{op}: channels must be a multiple of num_groups")
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"{op}: activation must be one of {', '.join(ACTIVATIONS)}")
+    if not eps >= 0.0:
+        raise ValueError(f"{op}: eps must be >= 0")
     for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None:
-            _refuse(op, (tuple(t.shape) == (x.size(-1),), f"{name} must have shape (C,)"),
-                    (t.dtype in (x.dtype, torch.float32), f"{name} must be float32 or of x's type"),
-                    (t.device == x.device, f"{name} must be on the same device as x"))
-    if weight is not None and bias is not None:
-        _refuse(op, (weight.dtype == bias.dtype, "weight and bias must have the same type"))
+        if t is None:
+            continue
+        if t.dim() != 1 or t.size(0) != x.size(-1):
+            raise ValueError(f"{op}: {name} must have shape (C,)")
+        if t.dtype != x.dtype and t.dtype != torch.float32:
+            raise ValueError(f"{op}: {name} must be float32 or of x's type")
+        if t.device != x.device:
+            raise ValueError(f"{op}: {name} must be on the same device as x")
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise ValueError(f"{op}: weight and bias must have the same type")
     if layout is not None:
         _check_layout(op, layout, "layout", x.device)
     clouds = layout.offsets.numel() - 1 if layout is not None else x.size(0) if x.dim() == 3 else 1
     if clouds == 0:
         return torch.empty_like(x)
-    rows = dense(x).reshape(-1, x.size(-1))
-    y = _GroupNorm.apply(rows, None if weight is None else dense(weight), None if bias is None else dense(bias),
-                         None if layout is None else layout.offsets, clouds, num_groups, float(eps),
-                         ACTIVATIONS.index(activation))
-    return y.reshape(x.shape)
+    rows = dense(x)
+    if x.dim() == 3:
+        rows = rows.reshape(-1, x.size(-1))
+    weight, bias = (None if t is None else dense(t) for t in (weight, bias))
+    offsets = None if layout is None else layout.offsets
+    number = ACTIVATIONS.index(activation)
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
+                                    or (bias is not None and bias.requires_grad)):
+        y = _GroupNorm.apply(rows, weight, bias, offsets, clouds, num_groups, float(eps), number)
+    else:
+        y = _C.group_norm(rows, offsets, clouds, num_groups, weight, bias, float(eps), number)[0]
+    return y if x.dim() == 2 else y.reshape(x.shape)

@@ -396,15 +396,13 @@ hipError_t launch(const AttendArgs& a, hipStream_t stream) {
     if (a.table != nullptr) {
         const auto kernel = attend_kernel<T, DP, RT, W, true>;
         const size_t lds = std::max(stage + bias, parts);
-        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                                 hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds));
+        const hipError_t e = allow_lds(kernel, lds);
         if (e != hipSuccess) return e;
         kernel<<<grid, kWave * W, lds, stream>>>(a, tiles, items);
     } else {
         const auto kernel = attend_kernel<T, DP, RT, W, false>;
         const size_t lds = std::max(stage, parts);
-        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                                 hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds));
+        const hipError_t e = allow_lds(kernel, lds);
         if (e != hipSuccess) return e;
         kernel<<<grid, kWave * W, lds, stream>>>(a, tiles, items);
     }

@@ -261,6 +261,14 @@ struct Slots {
     }
 };
 
+// Lets a kernel have this much dynamic LDS (64 KB needs no leave).
+template <typename K>
+hipError_t allow_lds(K kernel, size_t bytes) {
+    if (bytes <= 65536) return hipSuccess;
+    return hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                               static_cast<int>(bytes));
+}
+
 hipError_t launch_attend(const AttendArgs& a, bool bf16, hipStream_t stream);
 hipError_t launch_attend_backward(const AttendArgs& a, const AttendGrads& g, bool bf16, hipStream_t stream);
 // Parts of the table's gradient for these sizes.

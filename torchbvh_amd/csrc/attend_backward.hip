@@ -754,12 +754,6 @@ __global__ __launch_bounds__(kBlock) void invert_runs_kernel(const uint32_t* __r
     runs[b] = lo;
 }
 
-template <typename K>
-hipError_t allow_lds(K kernel, size_t bytes) {
-    return hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
-                               static_cast<int>(bytes));
-}
-
 template <typename T, int DP, int RT, bool kBias>
 hipError_t launch_dq(const AttendArgs& a, const AttendGrads& g, hipStream_t stream) {
     const int tiles = (a.q_block + RT * 16 - 1) / (RT * 16);
