@@ -45,26 +45,49 @@ struct Moments {
 __device__ __forceinline__ Moments join(Moments a, Moments b) {
     const float n = a.n + b.n;
     if (n == 0.0f) return a;
-    const float f = b.n / n, d = b.mean - a.mean;
+    const float f = b.n * __builtin_amdgcn_rcpf(n), d = b.mean - a.mean;
     return {n, a.mean + d * f, a.squares + b.squares + d * d * a.n * f};
 }
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// 1 / (1 + e^-z); the hardware's exponential and reciprocal are good to one unit in
+// the last place.
+__device__ __forceinline__ float sigmoid(float z) {
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -kLog2e));
+}
+
+// The normal distribution function at z, given bell = e^(-z^2 / 2), after Hastings,
+// "Approximations for Digital Computers" (1955), sheet 43: with x = |z| / sqrt 2 and
+// t = 1 / (1 + 0.3275911 x), erfc x = (a1 t + .. + a5 t^5) e^(-x^2) within 1.5e-7.
+__device__ __forceinline__ float normal_cdf(float z, float bell) {
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(fabsf(z), 0.3275911f * 0.70710678118654752f, 1.0f));
+    float p = __builtin_fmaf(t, 1.061405429f, -1.453152027f);
+    p = __builtin_fmaf(t, p, 1.421413741f);
+    p = __builtin_fmaf(t, p, -0.284496736f);
+    p = __builtin_fmaf(t, p, 0.254829592f);
+    const float tail = 0.5f * t * p * bell;
+    return z < 0.0f ? tail : 1.0f - tail;
+}
+__device__ __forceinline__ float bell_of(float z) { return __builtin_amdgcn_exp2f(z * z * (-0.5f * kLog2e)); }
 
 template <int kAct>
 __device__ __forceinline__ float activate(float z) {
     if constexpr (kAct == kRelu) return fmaxf(z, 0.0f);
-    if constexpr (kAct == kSilu) return z / (1.0f + __expf(-z));
-    if constexpr (kAct == kGelu) return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+    if constexpr (kAct == kSilu) return z * sigmoid(z);
+    if constexpr (kAct == kGelu) return z * normal_cdf(z, bell_of(z));
     return z;
 }
 template <int kAct>
 __device__ __forceinline__ float slope(float z) {
     if constexpr (kAct == kRelu) return z > 0.0f ? 1.0f : 0.0f;
     if constexpr (kAct == kSilu) {
-        const float s = 1.0f / (1.0f + __expf(-z));
-        return s * (1.0f + z * (1.0f - s));
+        const float s = sigmoid(z);
+        return s * __builtin_fmaf(z, 1.0f - s, 1.0f);
     }
     if constexpr (kAct == kGelu) {
-        return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * 0.39894228040143268f * __expf(-0.5f * z * z);
+        const float bell = bell_of(z);
+        return __builtin_fmaf(z * 0.39894228040143268f, bell, normal_cdf(z, bell));
     }
     return 1.0f;
 }
@@ -161,11 +184,13 @@ __global__ __launch_bounds__(kBlock) void norm_join_kernel(NormArgs a, int parts
     const int cloud = blockIdx.y, group = blockIdx.x, per = a.channels / a.groups;
     const float* in = a.parts + static_cast<int64_t>(cloud) * parts * a.channels * 2;
     Moments m = {0.0f, 0.0f, 0.0f};
+    const int64_t rows = slice_of(a, cloud, 0, 1).cloud_rows, each = (rows + parts - 1) / parts;
+    // A thread's slices of a channel at a time; neighbours take neighbouring channels.
     for (int i = threadIdx.x; i < parts * per; i += kBlock) {
         const int part = i / per, c = group * per + i - part * per;
-        const Slice s = slice_of(a, cloud, part, parts);
-        const float* p = in + (static_cast<int64_t>(part) * a.channels + c) * 2;
-        m = join(m, {static_cast<float>(s.last - s.first), p[0], p[1]});
+        const float2 p = *reinterpret_cast<const float2*>(in + (static_cast<int64_t>(part) * a.channels + c) * 2);
+        const int64_t here = min(max(rows - each * part, int64_t{0}), each);
+        m = join(m, {static_cast<float>(here), p.x, p.y});
     }
     m = join_across(m);
     if (lane_id() == 0) s_m[threadIdx.x / kWave] = m;
@@ -199,20 +224,34 @@ template <typename T, typename P, int V, int kAct>
 __global__ __launch_bounds__(kBlock) void norm_apply_kernel(NormArgs a) {
     const Place p = place<V>(a.channels);
     if (p.row < 0) return;
-    const Slice s = slice_of(a, blockIdx.y, blockIdx.x, gridDim.x);
+    // The slices from the last to the first: the end of what the launch before read is
+    // still in the memory-side cache.
+    const int cloud = a.clouds - 1 - blockIdx.y;
+    const Slice s = slice_of(a, cloud, gridDim.x - 1 - blockIdx.x, gridDim.x);
     Columns<P, V> c;
-    c.load(a, blockIdx.y, p.column);
+    c.load(a, cloud, p.column);
     const T* x = static_cast<const T*>(a.x) + p.column;
     T* y = static_cast<T*>(a.y) + p.column;
-    for (int64_t r = s.first + p.row; r < s.last; r += p.step) {
-        const Vec<T, V> v = *reinterpret_cast<const Vec<T, V>*>(x + r * a.channels);
-        Vec<T, V> o;
+    constexpr int kAhead = 4;  // rows loaded together
+    for (int64_t r = s.first + p.row; r < s.last; r += static_cast<int64_t>(p.step) * kAhead) {
+        Vec<T, V> v[kAhead];
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const float hat = (static_cast<float>(v.v[i]) - c.mean[i]) * c.rstd[i];
-            o.v[i] = static_cast<T>(activate<kAct>(__builtin_fmaf(hat, c.weight[i], c.bias[i])));
+        for (int j = 0; j < kAhead; ++j) {
+            const int64_t row = r + static_cast<int64_t>(j) * p.step;
+            if (row < s.last) v[j] = *reinterpret_cast<const Vec<T, V>*>(x + row * a.channels);
         }
-        *reinterpret_cast<Vec<T, V>*>(y + r * a.channels) = o;
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            const int64_t row = r + static_cast<int64_t>(j) * p.step;
+            if (row >= s.last) break;
+            Vec<T, V> o;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float hat = (static_cast<float>(v[j].v[i]) - c.mean[i]) * c.rstd[i];
+                o.v[i] = static_cast<T>(activate<kAct>(__builtin_fmaf(hat, c.weight[i], c.bias[i])));
+            }
+            *reinterpret_cast<Vec<T, V>*>(y + row * a.channels) = o;
+        }
     }
 }
 
@@ -231,15 +270,28 @@ __global__ __launch_bounds__(kBlock) void norm_sums_kernel(NormArgs a) {
         c.load(a, cloud, p.column);
         const T* x = static_cast<const T*>(a.x) + p.column;
         const T* up = static_cast<const T*>(a.grad) + p.column;
-        for (int64_t r = s.first + p.row; r < s.last; r += p.step) {
-            const Vec<T, V> v = *reinterpret_cast<const Vec<T, V>*>(x + r * a.channels);
-            const Vec<T, V> u = *reinterpret_cast<const Vec<T, V>*>(up + r * a.channels);
+        constexpr int kAhead = 4;
+        for (int64_t r = s.first + p.row; r < s.last; r += static_cast<int64_t>(p.step) * kAhead) {
+            Vec<T, V> v[kAhead], u[kAhead];
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const float hat = (static_cast<float>(v.v[i]) - c.mean[i]) * c.rstd[i];
-                const float dz = static_cast<float>(u.v[i]) * slope<kAct>(__builtin_fmaf(hat, c.weight[i], c.bias[i]));
-                sum[i] += dz;
-                hats[i] = __builtin_fmaf(dz, hat, hats[i]);
+            for (int j = 0; j < kAhead; ++j) {
+                const int64_t row = r + static_cast<int64_t>(j) * p.step;
+                if (row < s.last) {
+                    v[j] = *reinterpret_cast<const Vec<T, V>*>(x + row * a.channels);
+                    u[j] = *reinterpret_cast<const Vec<T, V>*>(up + row * a.channels);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) {
+                if (r + static_cast<int64_t>(j) * p.step >= s.last) break;
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const float hat = (static_cast<float>(v[j].v[i]) - c.mean[i]) * c.rstd[i];
+                    const float dz =
+                        static_cast<float>(u[j].v[i]) * slope<kAct>(__builtin_fmaf(hat, c.weight[i], c.bias[i]));
+                    sum[i] += dz;
+                    hats[i] = __builtin_fmaf(dz, hat, hats[i]);
+                }
             }
         }
     }
@@ -264,7 +316,9 @@ __global__ __launch_bounds__(kBlock) void norm_sums_kernel(NormArgs a) {
 }
 
 // One wave per (channel, cloud): the slices' sums, into `channel_sums`
-// (cloud, channel) -> (sum dz, sum dz xhat).
+// (cloud, channel) -> (sum dz, sum dz xhat), which for a single cloud are the
+// parameters' gradients.
+template <typename P>
 __global__ __launch_bounds__(kWave) void norm_channel_kernel(NormArgs a, int parts, float* __restrict__ channel_sums) {
     const int c = blockIdx.x, cloud = blockIdx.y;
     float x = 0.0f, y = 0.0f;
@@ -281,6 +335,10 @@ __global__ __launch_bounds__(kWave) void norm_channel_kernel(NormArgs a, int par
     if (lane_id() == 0) {
         channel_sums[(static_cast<int64_t>(cloud) * a.channels + c) * 2] = x;
         channel_sums[(static_cast<int64_t>(cloud) * a.channels + c) * 2 + 1] = y;
+        if (a.clouds == 1) {
+            if (a.dbias) static_cast<P*>(a.dbias)[c] = static_cast<P>(x);
+            if (a.dweight) static_cast<P*>(a.dweight)[c] = static_cast<P>(y);
+        }
     }
 }
 
@@ -308,8 +366,8 @@ template <typename T, typename P, int V, int kAct>
 __global__ __launch_bounds__(kBlock) void norm_dx_kernel(NormArgs a, const float* __restrict__ channel_sums) {
     const Place p = place<V>(a.channels);
     if (p.row < 0) return;
-    const int cloud = blockIdx.y;
-    const Slice s = slice_of(a, cloud, blockIdx.x, gridDim.x);
+    const int cloud = a.clouds - 1 - blockIdx.y;  // from the last slice to the first, as above
+    const Slice s = slice_of(a, cloud, gridDim.x - 1 - blockIdx.x, gridDim.x);
     if (s.first + p.row >= s.last) return;
     Columns<P, V> c;
     c.load(a, cloud, p.column);
@@ -339,17 +397,103 @@ __global__ __launch_bounds__(kBlock) void norm_dx_kernel(NormArgs a, const float
     const T* x = static_cast<const T*>(a.x) + p.column;
     const T* up = static_cast<const T*>(a.grad) + p.column;
     T* dx = static_cast<T*>(a.dx) + p.column;
-    for (int64_t r = s.first + p.row; r < s.last; r += p.step) {
-        const Vec<T, V> v = *reinterpret_cast<const Vec<T, V>*>(x + r * a.channels);
-        const Vec<T, V> u = *reinterpret_cast<const Vec<T, V>*>(up + r * a.channels);
-        Vec<T, V> o;
+    constexpr int kAhead = 2;
+    for (int64_t r = s.first + p.row; r < s.last; r += static_cast<int64_t>(p.step) * kAhead) {
+        Vec<T, V> v[kAhead], u[kAhead];
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const float hat = (static_cast<float>(v.v[i]) - c.mean[i]) * c.rstd[i];
-            const float dz = static_cast<float>(u.v[i]) * slope<kAct>(__builtin_fmaf(hat, c.weight[i], c.bias[i]));
-            o.v[i] = static_cast<T>(c.rstd[i] * (c.weight[i] * dz - mean[i] - hat * hats[i]));
+        for (int j = 0; j < kAhead; ++j) {
+            const int64_t row = r + static_cast<int64_t>(j) * p.step;
+            if (row < s.last) {
+                v[j] = *reinterpret_cast<const Vec<T, V>*>(x + row * a.channels);
+                u[j] = *reinterpret_cast<const Vec<T, V>*>(up + row * a.channels);
+            }
         }
-        *reinterpret_cast<Vec<T, V>*>(dx + r * a.channels) = o;
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            const int64_t row = r + static_cast<int64_t>(j) * p.step;
+            if (row >= s.last) break;
+            Vec<T, V> o;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float hat = (static_cast<float>(v[j].v[i]) - c.mean[i]) * c.rstd[i];
+                const float dz =
+                    static_cast<float>(u[j].v[i]) * slope<kAct>(__builtin_fmaf(hat, c.weight[i], c.bias[i]));
+                o.v[i] = static_cast<T>(c.rstd[i] *
+                                        __builtin_fmaf(c.weight[i], dz, -__builtin_fmaf(hat, hats[i], mean[i])));
+            }
+            *reinterpret_cast<Vec<T, V>*>(dx + row * a.channels) = o;
+        }
+    }
+}
+
+// One work-group per (group, cloud) whose values all fit its registers: mean, then
+// squares around it, then y, in one launch and one read.
+constexpr int kSmallThreads = 1024, kSmallVectors = 8;
+
+__device__ __forceinline__ float small_sum(float x, float* s_sum) {
+#pragma unroll
+    for (int d = kWave / 2; d > 0; d >>= 1) x += __shfl_xor(x, d, kWave);
+    __syncthreads();
+    if (lane_id() == 0) s_sum[threadIdx.x / kWave] = x;
+    __syncthreads();
+    float total = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kSmallThreads / kWave; ++w) total += s_sum[w];
+    return total;
+}
+
+template <typename T, typename P, int V, int kAct>
+__global__ __launch_bounds__(kSmallThreads) void norm_small_kernel(NormArgs a) {
+    __shared__ float s_sum[kSmallThreads / kWave];
+    const int cloud = blockIdx.y, group = blockIdx.x, per = a.channels / a.groups, wide = per / V;
+    const Slice s = slice_of(a, cloud, 0, 1);
+    const int vectors = static_cast<int>(s.cloud_rows) * wide;
+    const float n = static_cast<float>(vectors * V);
+    const T* x = static_cast<const T*>(a.x) + s.first * a.channels + group * per;
+    T* y = static_cast<T*>(a.y) + s.first * a.channels + group * per;
+    Vec<T, V> v[kSmallVectors];
+    float sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kSmallVectors; ++k) {
+        const int i = threadIdx.x + k * kSmallThreads, row = i / wide;
+        if (i < vectors) {
+            v[k] = *reinterpret_cast<const Vec<T, V>*>(x + static_cast<int64_t>(row) * a.channels + (i - row * wide) * V);
+#pragma unroll
+            for (int j = 0; j < V; ++j) sum += static_cast<float>(v[k].v[j]);
+        }
+    }
+    const float mean = small_sum(sum, s_sum) / n;
+    float squares = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kSmallVectors; ++k) {
+        if (threadIdx.x + k * kSmallThreads < vectors) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float d = static_cast<float>(v[k].v[j]) - mean;
+                squares = __builtin_fmaf(d, d, squares);
+            }
+        }
+    }
+    const float rstd = vectors > 0 ? 1.0f / sqrtf(small_sum(squares, s_sum) / n + a.eps) : 0.0f;
+    if (threadIdx.x == 0) {
+        a.mean[cloud * a.groups + group] = vectors > 0 ? mean : 0.0f;
+        a.rstd[cloud * a.groups + group] = rstd;
+    }
+#pragma unroll
+    for (int k = 0; k < kSmallVectors; ++k) {
+        const int i = threadIdx.x + k * kSmallThreads, row = i / wide;
+        if (i < vectors) {
+            const int c = (i - row * wide) * V;
+            Vec<T, V> o;
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float w = a.weight ? static_cast<float>(static_cast<const P*>(a.weight)[group * per + c + j]) : 1.0f;
+                const float b = a.bias ? static_cast<float>(static_cast<const P*>(a.bias)[group * per + c + j]) : 0.0f;
+                const float hat = (static_cast<float>(v[k].v[j]) - mean) * rstd;
+                o.v[j] = static_cast<T>(activate<kAct>(__builtin_fmaf(hat, w, b)));
+            }
+            *reinterpret_cast<Vec<T, V>*>(y + static_cast<int64_t>(row) * a.channels + c) = o;
+        }
     }
 }
 
@@ -360,6 +504,13 @@ dim3 strips(const NormArgs& a, int V, int parts) {
 
 template <typename T, typename P, int V, int kAct>
 hipError_t run_forward(const NormArgs& a, hipStream_t stream) {
+    const int per = a.channels / a.groups;
+    // The longest cloud a ragged call may hold is all its rows.
+    const int64_t longest = a.offsets != nullptr ? a.rows : a.rows / a.clouds;
+    if (per % V == 0 && longest <= kSmallThreads * kSmallVectors * V / per) {
+        norm_small_kernel<T, P, V, kAct><<<dim3(a.groups, a.clouds), kSmallThreads, 0, stream>>>(a);
+        return hipGetLastError();
+    }
     const int parts = norm_parts(a.rows, a.clouds, a.channels);
     const dim3 grid = strips(a, V, parts);
     norm_stats_kernel<T, V><<<grid, kBlock, 0, stream>>>(a);
@@ -374,8 +525,8 @@ hipError_t run_backward(const NormArgs& a, hipStream_t stream) {
     const dim3 grid = strips(a, V, parts);
     float* channel_sums = a.parts + static_cast<int64_t>(a.clouds) * parts * a.channels * 2;
     norm_sums_kernel<T, P, V, kAct><<<grid, kBlock, 0, stream>>>(a);
-    norm_channel_kernel<<<dim3(a.channels, a.clouds), kWave, 0, stream>>>(a, parts, channel_sums);
-    if (a.dweight || a.dbias) norm_weights_kernel<P><<<a.channels, kWave, 0, stream>>>(a, channel_sums);
+    norm_channel_kernel<P><<<dim3(a.channels, a.clouds), kWave, 0, stream>>>(a, parts, channel_sums);
+    if (a.clouds > 1 && (a.dweight || a.dbias)) norm_weights_kernel<P><<<a.channels, kWave, 0, stream>>>(a, channel_sums);
     if (a.dx) norm_dx_kernel<T, P, V, kAct><<<grid, kBlock, 0, stream>>>(a, channel_sums);
     return hipGetLastError();
 }
@@ -410,11 +561,11 @@ hipError_t run(const NormArgs& a, bool bf16, bool wide_weights, bool backward, h
 }  // namespace
 
 int norm_parts(int64_t rows, int clouds, int channels) {
-    // Slices of about 64 KB, and no more work-groups than fill the chip eight
-    // times over.
+    // Slices of 16,384 values or more, and no more work-groups than fill the chip
+    // four times over.
     const int64_t mean = (rows + clouds - 1) / clouds;
     const int64_t by_size = (mean * channels + 16383) / 16384;
-    const int64_t by_fill = std::max<int64_t>(1, 2048 / clouds);
+    const int64_t by_fill = std::max<int64_t>(1, 1024 / clouds);
     return static_cast<int>(std::max<int64_t>(1, std::min(by_size, by_fill)));
 }
 
