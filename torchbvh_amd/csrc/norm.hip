@@ -179,14 +179,16 @@ __device__ __forceinline__ Moments join_across(Moments m) {
 }
 
 // One work-group per (group, cloud): the slices' moments of the group's channels.
-__global__ __launch_bounds__(kBlock) void norm_join_kernel(NormArgs a, int parts) {
-    __shared__ Moments s_m[kBlock / kWave];
+constexpr int kJoinThreads = 1024;
+
+__global__ __launch_bounds__(kJoinThreads) void norm_join_kernel(NormArgs a, int parts) {
+    __shared__ Moments s_m[kJoinThreads / kWave];
     const int cloud = blockIdx.y, group = blockIdx.x, per = a.channels / a.groups;
     const float* in = a.parts + static_cast<int64_t>(cloud) * parts * a.channels * 2;
     Moments m = {0.0f, 0.0f, 0.0f};
     const int64_t rows = slice_of(a, cloud, 0, 1).cloud_rows, each = (rows + parts - 1) / parts;
     // A thread's slices of a channel at a time; neighbours take neighbouring channels.
-    for (int i = threadIdx.x; i < parts * per; i += kBlock) {
+    for (int i = threadIdx.x; i < parts * per; i += kJoinThreads) {
         const int part = i / per, c = group * per + i - part * per;
         const float2 p = *reinterpret_cast<const float2*>(in + (static_cast<int64_t>(part) * a.channels + c) * 2);
         const int64_t here = min(max(rows - each * part, int64_t{0}), each);
@@ -197,31 +199,34 @@ __global__ __launch_bounds__(kBlock) void norm_join_kernel(NormArgs a, int parts
     __syncthreads();
     if (threadIdx.x == 0) {
         m = s_m[0];
-        for (int w = 1; w < kBlock / kWave; ++w) m = join(m, s_m[w]);
+        for (int w = 1; w < kJoinThreads / kWave; ++w) m = join(m, s_m[w]);
         a.mean[cloud * a.groups + group] = m.mean;
         a.rstd[cloud * a.groups + group] = m.n > 0.0f ? 1.0f / sqrtf(m.squares / m.n + a.eps) : 0.0f;
     }
 }
 
-// A thread's channels: z = (x - mean) scale + shift.
+// A thread's channels: xhat = x rstd + centre, z = x scale + shift, one rounding
+// each (their errors are those of the mean's own rounding times rstd).
 template <typename P, int V>
 struct Columns {
-    float mean[V], rstd[V], weight[V], bias[V];
+    float rstd[V], centre[V], scale[V], shift[V];
     __device__ __forceinline__ void load(const NormArgs& a, int cloud, int column) {
         const int per = a.channels / a.groups;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             const int at = cloud * a.groups + (column + i) / per;
-            mean[i] = a.mean[at];
+            const float weight = a.weight ? static_cast<float>(static_cast<const P*>(a.weight)[column + i]) : 1.0f;
+            const float bias = a.bias ? static_cast<float>(static_cast<const P*>(a.bias)[column + i]) : 0.0f;
             rstd[i] = a.rstd[at];
-            weight[i] = a.weight ? static_cast<float>(static_cast<const P*>(a.weight)[column + i]) : 1.0f;
-            bias[i] = a.bias ? static_cast<float>(static_cast<const P*>(a.bias)[column + i]) : 0.0f;
+            centre[i] = -a.mean[at] * rstd[i];
+            scale[i] = rstd[i] * weight;
+            shift[i] = __builtin_fmaf(centre[i], weight, bias);
         }
     }
 };
 
 template <typename T, typename P, int V, int kAct>
-__global__ __launch_bounds__(kBlock) void norm_apply_kernel(NormArgs a) {
+__global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(4))) void norm_apply_kernel(NormArgs a) {
     const Place p = place<V>(a.channels);
     if (p.row < 0) return;
     // The slices from the last to the first: the end of what the launch before read is
@@ -247,8 +252,8 @@ __global__ __launch_bounds__(kBlock) void norm_apply_kernel(NormArgs a) {
             Vec<T, V> o;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const float hat = (static_cast<float>(v[j].v[i]) - c.mean[i]) * c.rstd[i];
-                o.v[i] = static_cast<T>(activate<kAct>(__builtin_fmaf(hat, c.weight[i], c.bias[i])));
+                const float z = __builtin_fmaf(static_cast<float>(v[j].v[i]), c.scale[i], c.shift[i]);
+                o.v[i] = static_cast<T>(activate<kAct>(z));
             }
             *reinterpret_cast<Vec<T, V>*>(y + row * a.channels) = o;
         }
@@ -257,7 +262,7 @@ __global__ __launch_bounds__(kBlock) void norm_apply_kernel(NormArgs a) {
 
 // parts: (cloud, part, channel) -> (sum dz, sum dz xhat).
 template <typename T, typename P, int V, int kAct>
-__global__ __launch_bounds__(kBlock) void norm_sums_kernel(NormArgs a) {
+__global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(4))) void norm_sums_kernel(NormArgs a) {
     __shared__ float s_sum[kBlock * V], s_hat[kBlock * V];
     const Place p = place<V>(a.channels);
     const int cloud = blockIdx.y, part = blockIdx.x, parts = gridDim.x;
@@ -270,7 +275,7 @@ __global__ __launch_bounds__(kBlock) void norm_sums_kernel(NormArgs a) {
         c.load(a, cloud, p.column);
         const T* x = static_cast<const T*>(a.x) + p.column;
         const T* up = static_cast<const T*>(a.grad) + p.column;
-        constexpr int kAhead = 4;
+        constexpr int kAhead = 2;
         for (int64_t r = s.first + p.row; r < s.last; r += static_cast<int64_t>(p.step) * kAhead) {
             Vec<T, V> v[kAhead], u[kAhead];
 #pragma unroll
@@ -286,9 +291,10 @@ __global__ __launch_bounds__(kBlock) void norm_sums_kernel(NormArgs a) {
                 if (r + static_cast<int64_t>(j) * p.step >= s.last) break;
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    const float hat = (static_cast<float>(v[j].v[i]) - c.mean[i]) * c.rstd[i];
+                    const float value = static_cast<float>(v[j].v[i]);
+                    const float hat = __builtin_fmaf(value, c.rstd[i], c.centre[i]);
                     const float dz =
-                        static_cast<float>(u[j].v[i]) * slope<kAct>(__builtin_fmaf(hat, c.weight[i], c.bias[i]));
+                        static_cast<float>(u[j].v[i]) * slope<kAct>(__builtin_fmaf(value, c.scale[i], c.shift[i]));
                     sum[i] += dz;
                     hats[i] = __builtin_fmaf(dz, hat, hats[i]);
                 }
@@ -363,7 +369,7 @@ __global__ __launch_bounds__(kWave) void norm_weights_kernel(NormArgs a, const f
 }
 
 template <typename T, typename P, int V, int kAct>
-__global__ __launch_bounds__(kBlock) void norm_dx_kernel(NormArgs a, const float* __restrict__ channel_sums) {
+__global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(4))) void norm_dx_kernel(NormArgs a, const float* __restrict__ channel_sums) {
     const Place p = place<V>(a.channels);
     if (p.row < 0) return;
     const int cloud = a.clouds - 1 - blockIdx.y;  // from the last slice to the first, as above
@@ -391,8 +397,9 @@ __global__ __launch_bounds__(kBlock) void norm_dx_kernel(NormArgs a, const float
             gm *= inverse;
             gh *= inverse;
         }
-        mean[i] = gm;
-        hats[i] = gh;
+        // -rstd (mean + xhat hats), as mean' + x hats'.
+        hats[i] = -c.rstd[i] * gh * c.rstd[i];
+        mean[i] = -c.rstd[i] * __builtin_fmaf(c.centre[i], gh, gm);
     }
     const T* x = static_cast<const T*>(a.x) + p.column;
     const T* up = static_cast<const T*>(a.grad) + p.column;
@@ -415,11 +422,10 @@ __global__ __launch_bounds__(kBlock) void norm_dx_kernel(NormArgs a, const float
             Vec<T, V> o;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const float hat = (static_cast<float>(v[j].v[i]) - c.mean[i]) * c.rstd[i];
+                const float value = static_cast<float>(v[j].v[i]);
                 const float dz =
-                    static_cast<float>(u[j].v[i]) * slope<kAct>(__builtin_fmaf(hat, c.weight[i], c.bias[i]));
-                o.v[i] = static_cast<T>(c.rstd[i] *
-                                        __builtin_fmaf(c.weight[i], dz, -__builtin_fmaf(hat, hats[i], mean[i])));
+                    static_cast<float>(u[j].v[i]) * slope<kAct>(__builtin_fmaf(value, c.scale[i], c.shift[i]));
+                o.v[i] = static_cast<T>(__builtin_fmaf(c.scale[i], dz, __builtin_fmaf(value, hats[i], mean[i])));
             }
             *reinterpret_cast<Vec<T, V>*>(dx + row * a.channels) = o;
         }
@@ -514,7 +520,7 @@ hipError_t run_forward(const NormArgs& a, hipStream_t stream) {
     const int parts = norm_parts(a.rows, a.clouds, a.channels);
     const dim3 grid = strips(a, V, parts);
     norm_stats_kernel<T, V><<<grid, kBlock, 0, stream>>>(a);
-    norm_join_kernel<<<dim3(a.groups, a.clouds), kBlock, 0, stream>>>(a, parts);
+    norm_join_kernel<<<dim3(a.groups, a.clouds), kJoinThreads, 0, stream>>>(a, parts);
     norm_apply_kernel<T, P, V, kAct><<<grid, kBlock, 0, stream>>>(a);
     return hipGetLastError();
 }
