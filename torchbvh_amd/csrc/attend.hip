@@ -130,43 +130,184 @@ __global__ __launch_bounds__(kWave* W) __attribute__((amdgpu_waves_per_eu(forwar
         v_at[i] = d < a.D ? static_cast<uint32_t>(p / (DP / 8) * a.v_row + d) * E : kNowhere;
     }
 
+    // A chosen block's rows, and the step that the loop is at.
+    const int k_bytes = static_cast<int>(a.k_row) * E, v_bytes = static_cast<int>(a.v_row) * E;
+    const int k_tail = static_cast<int>(a.k_row - a.D) * E, v_tail = static_cast<int>(a.v_row - a.D) * E;
+    Vec8<T> kf[KT][DS], vs[VL];
+    int cells[3] = {};
+    const char *k_first = nullptr, *v_first = nullptr;
+    const int32_t* cell_first = a.k_cells;
+    int ahead = 0;  // rows of the step that is loaded next
+
+    const auto load_keys = [&] {
+        const Buffer kb = buffer(k_first, max(ahead * k_bytes - k_tail, 0));
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int s = 0; s < DS; ++s) kf[kt][s] = load8<T>(kb, k_at[kt][s]);
+    };
+    const auto load_values = [&] {
+        const Buffer vb = buffer(v_first, max(ahead * v_bytes - v_tail, 0));
+#pragma unroll
+        for (int i = 0; i < VL; ++i) vs[i] = load8<T>(vb, v_at[i]);
+        if constexpr (kBias) {
+            // Three loads whatever the axes: the compiler counts what is outstanding, and a
+            // load that might not be there would have it wait for all of them.
+            const int32_t* at = ahead > 0 ? cell_first + min(lane & (kChunk - 1), ahead - 1) * a.axes : a.q_cells;
+#pragma unroll
+            for (int x = 0; x < 3; ++x) cells[x] = at[min(x, a.axes - 1)];
+        }
+    };
+
+    // One step over the keys and values that are loaded; `left` of them are there.
+    const auto take = [&](int left) {
+        f32x4 st[KT][RT];
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                st[kt][rt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int s = 0; s < DS; ++s) st[kt][rt] = mma(kf[kt][s], qf[rt][s], st[kt][rt]);
+            }
+        load_keys();
+        // Scores less the reference, in powers of two.
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) st[kt][rt][r] = __builtin_fmaf(st[kt][rt][r], to_log2, -ref[rt]);
+        if constexpr (kBias) {
+#pragma unroll
+            for (int x = 0; x < 3; ++x) {
+                if (x >= a.axes) continue;
+                const int mine = s_cell[x * kChunk + (lane & (kChunk - 1))];
+                const bool close = __all(static_cast<uint32_t>(mine - close_from[x]) <= static_cast<uint32_t>(close_span[x])) &&
+                                   close_span[x] >= 0;
+                const char* table = reinterpret_cast<const char*>(s_bias + x * span);
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) {
+                    const int4 kc = *reinterpret_cast<const int4*>(s_cell + x * kChunk + 16 * kt + 4 * g);
+                    const int key[4] = {kc.x, kc.y, kc.z, kc.w};
+                    if (close) {
+#pragma unroll
+                        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r)
+                                st[kt][rt][r] += *reinterpret_cast<const float*>(table + (bias_row[rt] + qc[rt][x] - key[r]));
+                    } else {
+#pragma unroll
+                        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r)
+                                st[kt][rt][r] += *reinterpret_cast<const float*>(
+                                    table + (bias_row[rt] + cell_distance(qc[rt][x], key[r], reach)));
+                    }
+                }
+            }
+        }
+        if (left < kChunk) {
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (16 * kt + 4 * g + r >= left)
+#pragma unroll
+                        for (int rt = 0; rt < RT; ++rt) st[kt][rt][r] = -INFINITY;
+        }
+        float most[RT];
+        bool above = false;
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            float m = fmaxf(fmaxf(st[0][rt][0], st[0][rt][1]), fmaxf(st[0][rt][2], st[0][rt][3]));
+#pragma unroll
+            for (int kt = 1; kt < KT; ++kt)
+                m = fmaxf(fmaxf(fmaxf(m, st[kt][rt][0]), fmaxf(st[kt][rt][1], st[kt][rt][2])), st[kt][rt][3]);
+            most[rt] = m;
+            above |= m > limit[rt];
+        }
+        if (__any(above)) {
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                // The largest score so far, and how far the reference follows: rows that
+                // have met no score above -inf keep a reference of 0 and weights of 0.
+                const float m = across_groups_max(most[rt]);
+                const float up = limit[rt] < 0.0f ? (m == -INFINITY ? 0.0f : m) : fmaxf(m, 0.0f);
+                if (m != -INFINITY) limit[rt] = kSlack;
+                const float keep = __builtin_amdgcn_exp2f(-up);
+                ref[rt] += up;
+                sum[rt] *= keep;
+                sums[rt] *= keep;
+#pragma unroll
+                for (int t = 0; t < DT; ++t) acc[rt][t] *= keep;
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) st[kt][rt][r] -= up;
+            }
+        }
+        // Weights are rounded to T for the product with v (2^-9 each in bf16,
+        // independent); the sums are of the same rounded weights, in fp32.
+        Vec8<T> pf[RT], lo[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) st[kt][rt][r] = __builtin_amdgcn_exp2f(st[kt][rt][r]);
+            pf[rt] = join<T>(st[0][rt], st[1][rt]);
+            if constexpr (kSumByProduct) {
+                sums[rt] = mma(ones, pf[rt], sums[rt]);
+                if (kBias && exact) {
+                    lo[rt] = join_left<T>(pf[rt], st[0][rt], st[1][rt]);
+                    sums[rt] = mma(ones, lo[rt], sums[rt]);
+                }
+            } else {
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt)
+                    sum[rt] += (st[kt][rt][0] + st[kt][rt][1]) + (st[kt][rt][2] + st[kt][rt][3]);
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < DT; ++t) {
+            const Vec8<T> vf = load_turned<T, LDV>(s_v, t, n, g);
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                acc[rt][t] = mma(vf, pf[rt], acc[rt][t]);
+                if (kSumByProduct && kBias && exact) acc[rt][t] = mma(vf, lo[rt], acc[rt][t]);
+            }
+        }
+    };
+
     for (int from = 0; from < a.count; from += kWave) {
         const int slots = min(a.count - from, kWave);
         Slots list;
         list.load(a.selected + group * a.count + from, slots, a.blocks, a.k_starts, a.k_block, a.k_total);
-        int slot = wave, base = 0;
-        Rows kr = {0, 0};
-        const auto skip = [&] {  // to the next chosen block that has rows
-            kr.count = 0;
-            while (slot < slots && (kr = list.at(slot)).count == 0) slot += W;
-        };
-        Vec8<T> kf[KT][DS], vs[VL];
-        int cells[3];
-        const auto load_keys = [&] {
-            const Buffer kb = rows_buffer<T>(a.k, kr.first + base, c * a.k_head, kr.count - base, a.k_row, a.D);
-#pragma unroll
-            for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-                for (int s = 0; s < DS; ++s) kf[kt][s] = load8<T>(kb, k_at[kt][s]);
-        };
-        const auto load_values = [&] {
-            const Buffer vb = rows_buffer<T>(a.v, kr.first + base, c * a.v_head, kr.count - base, a.v_row, a.D);
-#pragma unroll
-            for (int i = 0; i < VL; ++i) vs[i] = load8<T>(vb, v_at[i]);
-            if constexpr (kBias) {
-                const int64_t row = kr.first + base + min(lane & (kChunk - 1), max(kr.count - base - 1, 0));
-#pragma unroll
-                for (int x = 0; x < 3; ++x)
-                    if (x < a.axes) cells[x] = a.k_cells[row * a.axes + x];
+        int slot = wave - W, rows_left = 0;
+        const auto next = [&] {  // on by a step: 32 rows, or to the next chosen block that has rows
+            k_first += kChunk * k_bytes;
+            v_first += kChunk * v_bytes;
+            if constexpr (kBias) cell_first += kChunk * a.axes;
+            rows_left -= kChunk;
+            if (rows_left <= 0) {
+                Rows kr = {0, 0};
+                for (slot += W; slot < slots; slot += W) {
+                    kr = list.at(slot);
+                    if (kr.count > 0) break;
+                }
+                rows_left = slot < slots ? kr.count : 0;
+                k_first = reinterpret_cast<const char*>(static_cast<const T*>(a.k) + kr.first * a.k_row + c * a.k_head);
+                v_first = reinterpret_cast<const char*>(static_cast<const T*>(a.v) + kr.first * a.v_row + c * a.v_head);
+                if constexpr (kBias) cell_first = a.k_cells + kr.first * a.axes;
             }
+            ahead = rows_left;  // past the last block: nothing, whose loads give zeros
         };
-        skip();
-        if (slot < slots) {
-            load_values();
-            load_keys();
-        }
-        while (slot < slots) {
-            const int left = kr.count - base;
+        next();
+        load_values();
+        load_keys();
+        while (ahead > 0) {
+            const int left = ahead;
             wave_sync();
 #pragma unroll
             for (int i = 0; i < VL; ++i) {
@@ -175,139 +316,14 @@ __global__ __launch_bounds__(kWave* W) __attribute__((amdgpu_waves_per_eu(forwar
             }
             if constexpr (kBias) {
 #pragma unroll
-                for (int x = 0; x < 3; ++x)
-                    if (x < a.axes) s_cell[x * kChunk + (lane & (kChunk - 1))] = cell_bytes(cells[x]);
+                for (int x = 0; x < 3; ++x) s_cell[x * kChunk + (lane & (kChunk - 1))] = cell_bytes(cells[x]);
             }
             wave_sync();
-            base += kChunk;
-            if (base >= kr.count) {
-                base = 0;
-                slot += W;
-                skip();
-            }
-            if (slot < slots) load_values();
-            f32x4 st[KT][RT];
-#pragma unroll
-            for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
-                    st[kt][rt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                    for (int s = 0; s < DS; ++s) st[kt][rt] = mma(kf[kt][s], qf[rt][s], st[kt][rt]);
-                }
-            if (slot < slots) load_keys();
-            // Scores less the reference, in powers of two.
-#pragma unroll
-            for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) st[kt][rt][r] = __builtin_fmaf(st[kt][rt][r], to_log2, -ref[rt]);
-            if constexpr (kBias) {
-#pragma unroll
-                for (int x = 0; x < 3; ++x) {
-                    if (x >= a.axes) continue;
-                    const int mine = s_cell[x * kChunk + (lane & (kChunk - 1))];
-                    const bool close = __all(static_cast<uint32_t>(mine - close_from[x]) <= static_cast<uint32_t>(close_span[x])) &&
-                                       close_span[x] >= 0;
-                    const char* table = reinterpret_cast<const char*>(s_bias + x * span);
-#pragma unroll
-                    for (int kt = 0; kt < KT; ++kt) {
-                        const int4 kc = *reinterpret_cast<const int4*>(s_cell + x * kChunk + 16 * kt + 4 * g);
-                        const int key[4] = {kc.x, kc.y, kc.z, kc.w};
-                        if (close) {
-#pragma unroll
-                            for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                                for (int r = 0; r < 4; ++r)
-                                    st[kt][rt][r] += *reinterpret_cast<const float*>(table + (bias_row[rt] + qc[rt][x] - key[r]));
-                        } else {
-#pragma unroll
-                            for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                                for (int r = 0; r < 4; ++r)
-                                    st[kt][rt][r] += *reinterpret_cast<const float*>(
-                                        table + (bias_row[rt] + cell_distance(qc[rt][x], key[r], reach)));
-                        }
-                    }
-                }
-            }
-            if (left < kChunk) {
-#pragma unroll
-                for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (16 * kt + 4 * g + r >= left)
-#pragma unroll
-                            for (int rt = 0; rt < RT; ++rt) st[kt][rt][r] = -INFINITY;
-            }
-            float most[RT];
-            bool above = false;
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                float m = fmaxf(fmaxf(st[0][rt][0], st[0][rt][1]), fmaxf(st[0][rt][2], st[0][rt][3]));
-#pragma unroll
-                for (int kt = 1; kt < KT; ++kt)
-                    m = fmaxf(fmaxf(fmaxf(m, st[kt][rt][0]), fmaxf(st[kt][rt][1], st[kt][rt][2])), st[kt][rt][3]);
-                most[rt] = m;
-                above |= m > limit[rt];
-            }
-            if (__any(above)) {
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
-                    // The largest score so far, and how far the reference follows: rows that
-                    // have met no score above -inf keep a reference of 0 and weights of 0.
-                    const float m = across_groups_max(most[rt]);
-                    const float up = limit[rt] < 0.0f ? (m == -INFINITY ? 0.0f : m) : fmaxf(m, 0.0f);
-                    if (m != -INFINITY) limit[rt] = kSlack;
-                    const float keep = __builtin_amdgcn_exp2f(-up);
-                    ref[rt] += up;
-                    sum[rt] *= keep;
-                    sums[rt] *= keep;
-#pragma unroll
-                    for (int t = 0; t < DT; ++t) acc[rt][t] *= keep;
-#pragma unroll
-                    for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) st[kt][rt][r] -= up;
-                }
-            }
-            // Weights are rounded to T for the product with v (2^-9 each in bf16,
-            // independent); the sums are of the same rounded weights, in fp32.
-            Vec8<T> pf[RT], lo[RT];
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-#pragma unroll
-                for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) st[kt][rt][r] = __builtin_amdgcn_exp2f(st[kt][rt][r]);
-            }
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                pf[rt] = join<T>(st[0][rt], st[1][rt]);
-                if constexpr (kSumByProduct) {
-                    sums[rt] = mma(ones, pf[rt], sums[rt]);
-                    if (kBias && exact) {
-#pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            lo[rt][j] = static_cast<T>(st[j / 4][rt][j % 4] - static_cast<float>(pf[rt][j]));
-                        sums[rt] = mma(ones, lo[rt], sums[rt]);
-                    }
-                } else {
-#pragma unroll
-                    for (int kt = 0; kt < KT; ++kt)
-                        sum[rt] += (st[kt][rt][0] + st[kt][rt][1]) + (st[kt][rt][2] + st[kt][rt][3]);
-                }
-            }
-#pragma unroll
-            for (int t = 0; t < DT; ++t) {
-                const Vec8<T> vf = load_turned<T, LDV>(s_v, t, n, g);
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
-                    acc[rt][t] = mma(vf, pf[rt], acc[rt][t]);
-                    if (kSumByProduct && kBias && exact) acc[rt][t] = mma(vf, lo[rt], acc[rt][t]);
-                }
-            }
+            next();
+            // With a bias the compiler orders the loads better behind a branch (16 x 10,000
+            // points: 212 us, 257 without).
+            if (!kBias || ahead > 0) load_values();
+            take(left);
         }
     }
 
