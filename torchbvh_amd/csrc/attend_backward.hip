@@ -35,6 +35,12 @@ __device__ __forceinline__ int least_of(int v, uint32_t todo) {
     return min(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16));
 }
 
+// The value of another lane of the row of 16 (shifted by a DPP control), 0 past its ends.
+template <int kControl>
+__device__ __forceinline__ float row_lane(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), kControl, 0xf, 0xf, true));
+}
+
 // Unit vectors as a fragment: slot j is 1 where row j's cell is `at`.
 template <typename T>
 __device__ __forceinline__ Vec8<T> units(const int* cells, int g, int at) {
@@ -331,12 +337,17 @@ __global__ __launch_bounds__(kWave)
                                 }
                                 // sums[r]: query cell q_low + 4 g + r, key cell k_low + n.
                                 const int apart = min(max((q_low - k_low) / 4, -(a.reach + kWindow)), a.reach + kWindow);
+                                // Distance 4 g - m of the window gathers sums[r] of lanes n = m + r: for
+                                // m >= 0 on lane m, for m = -3 .. -1 on lane m + 16.
+                                const float here_sum = ((sums[0] + row_lane<0x101>(sums[1])) + row_lane<0x102>(sums[2])) +
+                                                       row_lane<0x103>(sums[3]);
+                                const float wrapped = (row_lane<0x11f>(sums[1]) + row_lane<0x11e>(sums[2])) +
+                                                      row_lane<0x11d>(sums[3]);
                                 float* to = s_sum + (x * 4 + g) * wide + apart + a.reach + 2 * kWindow - 1 + 4 * g - n;
-#pragma unroll
-                                for (int r = 0; r < 4; ++r) {
-                                    to[r] += sums[r];
-                                    wave_sync();
-                                }
+                                const float first_sum = to[0], other_sum = n >= 13 ? to[16] : 0.0f;
+                                to[0] = first_sum + here_sum;
+                                if (n >= 13) to[16] = other_sum + wrapped;
+                                wave_sync();
                                 // On to the window that starts at the least cell after this one.
                                 q_low += 4 * kWindow;
                                 if (q_low > q_most[x]) break;

@@ -104,15 +104,18 @@ struct Best {
     __device__ __forceinline__ bool key_empty() const { return __ballot(key != kNoBlock) == 0; }
 };
 
-// One wave per block of queries.  With kCoarse it scores the boxes of 64 blocks
-// first, takes the nearest of them, and then only those that can still hold one of
-// the `count` least.
-template <int D, bool kCoarse>
-__global__ __launch_bounds__(kWave) void select_kernel(SelectArgs a) {
+// A block of queries: the centre of its box, and its cloud's blocks [first, last).
+template <int D>
+struct Asked {
+    float centre[D];
+    int64_t first, last;
+};
+template <int D>
+__device__ __forceinline__ Asked<D> asked(const SelectArgs& a, int64_t group) {
     const int lane = lane_id();
-    const int64_t group = blockIdx.x;
     const Rows rows = block_rows(a.q_starts, group, a.q_block, a.q_total);
-    float lo[D], hi[D], centre[D];
+    Asked<D> q;
+    float lo[D], hi[D];
 #pragma unroll
     for (int x = 0; x < D; ++x) {
         lo[x] = INFINITY;
@@ -127,21 +130,38 @@ __global__ __launch_bounds__(kWave) void select_kernel(SelectArgs a) {
         }
     }
 #pragma unroll
-    for (int x = 0; x < D; ++x) centre[x] = 0.5f * wave_min(lo[x]) + 0.5f * wave_max(hi[x]);
-
+    for (int x = 0; x < D; ++x) q.centre[x] = 0.5f * wave_min(lo[x]) + 0.5f * wave_max(hi[x]);
     const int cloud = cloud_of(a.q_clouds, a.clouds, group);
-    const int64_t first = cloud < 0 ? 0 : max(a.k_clouds[cloud], int64_t{0});
-    const int64_t last = cloud < 0 ? 0 : min(a.k_clouds[cloud + 1], static_cast<int64_t>(a.blocks));
+    q.first = cloud < 0 ? 0 : max(a.k_clouds[cloud], int64_t{0});
+    q.last = cloud < 0 ? 0 : min(a.k_clouds[cloud + 1], static_cast<int64_t>(a.blocks));
+    return q;
+}
+
+// The keys of blocks b0 .. b0 + 63, a lane each.
+template <int D>
+__device__ __forceinline__ uint64_t block_key(const SelectArgs& a, const Asked<D>& q, int64_t b0) {
+    const int64_t b = b0 + lane_id();
+    if (b < q.first || b >= q.last) return kNoBlock;
+    const float score = box_score<D>(a.boxes + b * 2 * D, q.centre);
+    return score < INFINITY ? static_cast<uint64_t>(__float_as_uint(score)) << 32 | static_cast<uint32_t>(b) : kNoBlock;
+}
+
+__device__ __forceinline__ void store_choice(const SelectArgs& a, int64_t group, uint64_t key) {
+    if (lane_id() < a.count) a.out[group * a.count + lane_id()] = key == kNoBlock ? -1 : static_cast<int32_t>(key);
+}
+
+// One wave per block of queries.  With kCoarse it scores the boxes of 64 blocks
+// first and visits these sets from the nearest on, until none can hold one of the
+// `count` least any more (one million points, 16,384 blocks of queries,
+// count 32: 97 us; the nearest set first and the others in their own order 196).
+template <int D, bool kCoarse>
+__global__ __launch_bounds__(kWave) void select_kernel(SelectArgs a) {
+    const int lane = lane_id();
+    const int64_t group = blockIdx.x;
+    const Asked<D> q = asked<D>(a, group);
+    const int64_t first = q.first, last = q.last;
     Best best;
-    const auto visit = [&](int64_t b0) {
-        const int64_t b = b0 + lane;
-        uint64_t key = kNoBlock;
-        if (b >= first && b < last) {
-            const float score = box_score<D>(a.boxes + b * 2 * D, centre);
-            if (score < INFINITY) key = static_cast<uint64_t>(__float_as_uint(score)) << 32 | static_cast<uint32_t>(b);
-        }
-        best.take(key, a.count);
-    };
+    const auto visit = [&](int64_t b0) { best.take(block_key<D>(a, q, b0), a.count); };
     if constexpr (!kCoarse) {
         for (int64_t b = first; b < last; b += kWave) visit(b);
     } else if (first < last) {
@@ -150,31 +170,56 @@ __global__ __launch_bounds__(kWave) void select_kernel(SelectArgs a) {
         const auto bound = [&](int64_t set) {
             uint64_t key = kNoBlock;
             if (set < end) {
-                const float score = box_score<D>(a.coarse + set * 2 * D, centre);
+                const float score = box_score<D>(a.coarse + set * 2 * D, q.centre);
                 if (score < INFINITY)
                     key = static_cast<uint64_t>(__float_as_uint(score)) << 32 | static_cast<uint32_t>(set * kWave);
             }
             return key;
         };
-        uint64_t nearest = kNoBlock;
-        for (int64_t s = begin; s < end; s += kWave) nearest = keep(nearest, bound(s + lane), true);
-#pragma unroll
-        for (int j = 1; j < kWave; j <<= 1) nearest = keep(nearest, shfl64(nearest, lane ^ j), true);
-        if (nearest != kNoBlock) {
-            const int64_t chosen = static_cast<uint32_t>(nearest) / kWave;
-            visit(chosen * kWave);
+        // The 64 nearest sets in order, until one is past the last block that counts;
+        // then whatever sets come after those 64, in their own order.
+        Best sets;
+        for (int64_t s = begin; s < end; s += kWave) sets.take(bound(s + lane), kWave);
+        int at = 0;
+        uint64_t key = kNoBlock;
+        for (; at < kWave; ++at) {
+            key = shfl64(sets.key, at);
+            if (key >= best.limit) break;
+            visit(static_cast<uint32_t>(key));
+        }
+        if (at == kWave) {
+            const uint64_t done = key;
             for (int64_t s = begin; s < end; s += kWave) {
-                const uint64_t key = bound(s + lane);
-                for (uint64_t todo = __ballot(key < best.limit && s + lane != chosen); todo != 0;) {
-                    const int at = __builtin_ctzll(todo);
-                    visit((s + at) * kWave);
+                const uint64_t mine = bound(s + lane);
+                for (uint64_t todo = __ballot(mine > done && mine < best.limit); todo != 0;) {
+                    const int next = __builtin_ctzll(todo);
+                    visit((s + next) * kWave);
                     todo &= todo - 1;
-                    todo &= __ballot(key < best.limit);
+                    todo &= __ballot(mine < best.limit);
                 }
             }
         }
     }
-    if (lane < a.count) a.out[group * a.count + lane] = best.key == kNoBlock ? -1 : static_cast<int32_t>(best.key);
+    store_choice(a, group, best.key);
+}
+
+// Few blocks of queries: sixteen waves each, which take every sixteenth 64 blocks
+// and merge what they kept.
+constexpr int kTeam = 16;
+template <int D>
+__global__ __launch_bounds__(kTeam* kWave) void select_team_kernel(SelectArgs a) {
+    __shared__ uint64_t s_key[kTeam][kWave];
+    const int lane = lane_id(), wave = threadIdx.x / kWave;
+    const Asked<D> q = asked<D>(a, blockIdx.x);
+    Best best;
+    for (int64_t b = q.first + wave * kWave; b < q.last; b += kTeam * kWave) best.take(block_key<D>(a, q, b), a.count);
+    for (int half = kTeam / 2; half > 0; half >>= 1) {
+        s_key[wave][lane] = best.key;
+        __syncthreads();
+        if (wave < half) best.key = merged(best.key, s_key[wave + half][lane]);
+        __syncthreads();
+    }
+    if (wave == 0) store_choice(a, blockIdx.x, best.key);
 }
 
 }  // namespace
@@ -182,10 +227,17 @@ __global__ __launch_bounds__(kWave) void select_kernel(SelectArgs a) {
 namespace {
 // From this many blocks on the extra launch and level pay.
 constexpr int kCoarseBlocks = 512;
+// Where all teams together have few 64s to score, they are faster than one wave each
+// and the level of 64s with its launch (calls, us: 16 or 512 probes of 1,024 blocks 15
+// against 23; of 4,096 blocks 128 probes 15.6 against 17.7, 512 26 against 18).
+constexpr int kTeamBlocks = 4096;
+constexpr int64_t kTeamWork = 512 * 1024;  // (block of queries, block) pairs
 
 template <int D>
 hipError_t launch(const SelectArgs& a, hipStream_t stream) {
-    if (a.blocks >= kCoarseBlocks) {
+    if (a.blocks <= kTeamBlocks && int64_t{a.groups} * a.blocks <= kTeamWork) {
+        select_team_kernel<D><<<a.groups, kTeam * kWave, 0, stream>>>(a);
+    } else if (a.blocks >= kCoarseBlocks) {
         coarse_kernel<D><<<(a.blocks + kWave - 1) / kWave, kWave, 0, stream>>>(a.boxes, a.blocks, a.coarse);
         select_kernel<D, true><<<a.groups, kWave, 0, stream>>>(a);
     } else {
