@@ -569,9 +569,9 @@ int tbvh_select_blocks(const float* queries, int64_t q_rows, const int64_t* q_st
  * at most 256, heads / kv_heads * axes * (2 reach + 1) at most 4096.
  *
  * lse (heads, q_rows), the base-2 logarithm of each row's sum, wanted for the
- * backward, may be null.  rest (like out), in bf16 with a bias: what out's rounding
- * left off, of weights that are not rounded to bf16; without it (null) the table's
- * gradient is good to out's own precision only. */
+ * backward, may be null.  rest (like out), in bf16: what out's rounding left off, of
+ * weights that are not rounded to bf16; without it (null) the gradients are good to
+ * out's own precision only. */
 typedef struct tbvh_attend_args {
     const void *q, *k, *v;
     int64_t q_row_stride, q_head_stride, k_row_stride, k_head_stride, v_row_stride, v_head_stride;

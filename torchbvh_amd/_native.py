@@ -1283,11 +1283,11 @@ class _NativeOps:
         """`tbvh_attend`: q (rows, heads, D), k and v (rows, kv_heads, D) with
         contiguous channels; `bias` None or (table, map, q_cells, k_cells).
         Returns the output and, if wanted, its log-sum-exp in base 2 and, in
-        bfloat16 with a bias, what the output's rounding left off."""
+        bfloat16, what the output's rounding left off."""
         args = _attend_args("attend", q, k, v, selected, q_starts, k_starts, q_block, k_block, scale, bias)
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         lse = torch.empty((q.size(1), q.size(0)), dtype=torch.float32, device=q.device) if want_lse else None
-        rest = torch.empty_like(out) if want_lse and bias is not None and q.dtype == torch.bfloat16 else None
+        rest = torch.empty_like(out) if want_lse and q.dtype == torch.bfloat16 else None
         args.out, args.lse, args.rest = out.data_ptr(), lse.data_ptr() if want_lse else None, _address(rest)
         with _on(q.device):
             _check(load().tbvh_attend(ctypes.byref(args), _stream(q.device)))

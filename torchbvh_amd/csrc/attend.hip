@@ -29,8 +29,8 @@ constexpr int forward_waves(int DP, int RT, int W, bool bias) {
 // A wave holds its queries and sums in registers, takes 32 keys a step straight
 // into the first product's fragments, and turns the values' rows through LDS.
 // The next step's keys and values are loaded while this one's are used.
-template <typename T, int DP, int RT, int W, bool kBias>
-__global__ __launch_bounds__(kWave* W) __attribute__((amdgpu_waves_per_eu(forward_waves<T>(DP, RT, W, kBias)))) void attend_kernel(AttendArgs a, int tiles, int64_t items) {
+template <typename T, int DP, int RT, int W, bool kBias, bool kExact>
+__global__ __launch_bounds__(kWave* W) __attribute__((amdgpu_waves_per_eu(forward_waves<T>(DP, RT, W, kBias || kExact)))) void attend_kernel(AttendArgs a, int tiles, int64_t items) {
     constexpr int DS = DP / 32, DT = DP / 16, KT = kChunk / 16, E = sizeof(T);
     constexpr int LDV = turned_stride<T>(DP);
     constexpr int VL = kChunk * DP / 8 / kWave;  // 8-value pieces of a lane
@@ -107,10 +107,10 @@ __global__ __launch_bounds__(kWave* W) __attribute__((amdgpu_waves_per_eu(forwar
 #pragma unroll
         for (int t = 0; t < DT; ++t) acc[rt][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    // A table's gradient is a sum in which each row's scores cancel, down to the
-    // error of delta = grad . out; so where it is wanted the weights take part with
-    // what their rounding left off, too, and so is the output kept.
-    const bool exact = a.rest != nullptr;
+    // kExact, in bf16 where gradients are wanted: ds = p (dp - delta) takes over the
+    // error of delta = grad . out, in a table's gradient for whole rows at once.  So the
+    // weights then take part with what their rounding left off, too, and so is the
+    // output kept (`rest`).
     Vec8<T> ones;
 #pragma unroll
     for (int j = 0; j < 8; ++j) ones[j] = static_cast<T>(1.0f);
@@ -259,7 +259,7 @@ __global__ __launch_bounds__(kWave* W) __attribute__((amdgpu_waves_per_eu(forwar
             pf[rt] = join<T>(st[0][rt], st[1][rt]);
             if constexpr (kSumByProduct) {
                 sums[rt] = mma(ones, pf[rt], sums[rt]);
-                if (kBias && exact) {
+                if constexpr (kExact) {
                     lo[rt] = join_left<T>(pf[rt], st[0][rt], st[1][rt]);
                     sums[rt] = mma(ones, lo[rt], sums[rt]);
                 }
@@ -275,7 +275,7 @@ __global__ __launch_bounds__(kWave* W) __attribute__((amdgpu_waves_per_eu(forwar
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
                 acc[rt][t] = mma(vf, pf[rt], acc[rt][t]);
-                if (kSumByProduct && kBias && exact) acc[rt][t] = mma(vf, lo[rt], acc[rt][t]);
+                if constexpr (kExact) acc[rt][t] = mma(vf, lo[rt], acc[rt][t]);
             }
         }
     };
@@ -384,7 +384,7 @@ __global__ __launch_bounds__(kWave* W) __attribute__((amdgpu_waves_per_eu(forwar
 #pragma unroll
                 for (int r = 0; r < 4; ++r) o[r] = static_cast<T>(acc[rt][t][r] * inverse);
                 *reinterpret_cast<Vec4<T>*>(row + d) = o;
-                if (kSumByProduct && kBias && exact) {
+                if constexpr (kExact) {
                     Vec4<T> left;
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
@@ -409,20 +409,21 @@ hipError_t launch(const AttendArgs& a, hipStream_t stream) {
     const size_t bias = static_cast<size_t>(W) * 3 * kChunk * sizeof(int) +
                         static_cast<size_t>(a.share) * a.axes * (2 * a.reach + 1) * sizeof(float);
     const size_t parts = W > 1 ? static_cast<size_t>(W) * RT * (DP / 16 * 4 + 2) * kWave * sizeof(float) : 0;
-    if (a.table != nullptr) {
-        const auto kernel = attend_kernel<T, DP, RT, W, true>;
-        const size_t lds = std::max(stage + bias, parts);
+    const size_t lds = std::max(stage + (a.table != nullptr ? bias : 0), parts);
+    const auto run = [&](auto kernel) {
         const hipError_t e = allow_lds(kernel, lds);
         if (e != hipSuccess) return e;
         kernel<<<grid, kWave * W, lds, stream>>>(a, tiles, items);
-    } else {
-        const auto kernel = attend_kernel<T, DP, RT, W, false>;
-        const size_t lds = std::max(stage, parts);
-        const hipError_t e = allow_lds(kernel, lds);
-        if (e != hipSuccess) return e;
-        kernel<<<grid, kWave * W, lds, stream>>>(a, tiles, items);
+        return hipGetLastError();
+    };
+    if constexpr (sizeof(T) == 2) {
+        if (a.rest != nullptr) {
+            return a.table != nullptr ? run(attend_kernel<T, DP, RT, W, true, true>)
+                                      : run(attend_kernel<T, DP, RT, W, false, true>);
+        }
     }
-    return hipGetLastError();
+    return a.table != nullptr ? run(attend_kernel<T, DP, RT, W, true, false>)
+                              : run(attend_kernel<T, DP, RT, W, false, false>);
 }
 
 // Row tiles: 16 rows where a block has no more, else 64, or 32 where the

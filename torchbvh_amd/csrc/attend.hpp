@@ -174,7 +174,7 @@ struct AttendArgs {
     int axes = 0, buckets = 0, reach = 0;
     void* out = nullptr;   // (q_total, heads, D)
     float* lse = nullptr;  // (heads, q_total), base 2; null: not wanted
-    void* rest = nullptr;  // like out: what out's rounding left off (bf16 with a bias); null: not wanted
+    void* rest = nullptr;  // like out: what out's rounding left off (bf16); null: not wanted
 };
 
 struct AttendGrads {

@@ -135,7 +135,7 @@ __global__ __launch_bounds__(kWave)
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
                     dot = __builtin_fmaf(static_cast<float>(gf[rt][s][j]), static_cast<float>(o[j]), dot);
-                if (kBias && a.rest != nullptr) {
+                if (E == 2 && a.rest != nullptr) {
                     const Vec8<T> left = load8(static_cast<const T*>(a.rest) + (row * a.heads + h) * a.D, 32 * s + 8 * g,
                                                a.D, real);
 #pragma unroll
