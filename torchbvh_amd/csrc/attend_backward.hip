@@ -143,9 +143,9 @@ __global__ __launch_bounds__(kWave)
                         dot = __builtin_fmaf(static_cast<float>(gf[rt][s][j]), static_cast<float>(left[j]), dot);
                 }
             }
-            // A row that is not there has q = grad = 0: ds is 0 whatever its weight.
+            // A row that is not there weighs nothing, however large its bias.
             delta[rt] = across_groups_sum(dot);
-            lse[rt] = real ? a.lse[h * a.q_total + row] : 0.0f;
+            lse[rt] = real ? a.lse[h * a.q_total + row] : HUGE_VALF;
             if (real && g == 0) gr.delta[h * a.q_total + row] = delta[rt];
         }
         if constexpr (kBias) {
@@ -539,10 +539,12 @@ __global__ __launch_bounds__(kWave* W)
                         qf[rt][s] = load8<T>(qb, q_at[rt][s]);
                         gf[rt][s] = load8<T>(gb, g_at[rt][s]);
                     }
-                // Rows that are not there have q = grad = 0, so nothing comes of theirs.
+                // Rows that are not there have q = grad = 0 and weigh nothing: against a
+                // neighbour's lse their score of 0 could be past the largest float.
                 const int64_t mine = min(max(row + min(lane & (kStep - 1), here - 1), int64_t{0}), a.q_total - 1);
-                lse = a.lse[h * a.q_total + mine];
-                delta = gr.delta[h * a.q_total + mine];
+                const bool real = (lane & (kStep - 1)) < here;
+                lse = real ? a.lse[h * a.q_total + mine] : HUGE_VALF;
+                delta = real ? gr.delta[h * a.q_total + mine] : 0.0f;
                 if constexpr (kBias) {
                     head = hs * entries * 4;
 #pragma unroll
@@ -574,8 +576,8 @@ __global__ __launch_bounds__(kWave* W)
                     }
                 }
                 const int64_t mine = find(step * kStep + (lane & (kStep - 1)), h, real);
-                lse = a.lse[h * a.q_total + mine];
-                delta = gr.delta[h * a.q_total + mine];
+                lse = real ? a.lse[h * a.q_total + mine] : HUGE_VALF;
+                delta = real ? gr.delta[h * a.q_total + mine] : 0.0f;
                 if constexpr (kBias) {
                     head = (h - c * a.share) * entries * 4;
 #pragma unroll
