@@ -233,9 +233,11 @@ __global__ __launch_bounds__(kWave* W) __attribute__((amdgpu_waves_per_eu(forwar
                 // The largest score so far, and how far the reference follows: rows that
                 // have met no score above -inf keep a reference of 0 and weights of 0.
                 const float m = across_groups_max(most[rt]);
-                const float up = limit[rt] < 0.0f ? (m == -INFINITY ? 0.0f : m) : fmaxf(m, 0.0f);
+                const bool first = limit[rt] < 0.0f;
+                const float up = first ? (m == -INFINITY ? 0.0f : m) : fmaxf(m, 0.0f);
                 if (m != -INFINITY) limit[rt] = kSlack;
-                const float keep = __builtin_amdgcn_exp2f(-up);
+                // The sums are 0 before the first score, which may be far below 0.
+                const float keep = first ? 0.0f : __builtin_amdgcn_exp2f(-up);
                 ref[rt] += up;
                 sum[rt] *= keep;
                 sums[rt] *= keep;
