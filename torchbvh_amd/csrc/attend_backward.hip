@@ -21,8 +21,17 @@ constexpr int kTableWaves = 2048;
 
 constexpr int64_t kSplitWaves = 1 << 16;
 
-// Tiles of 16 query rows of a wave.
-constexpr int query_tiles(int size, int DP, int q_block) { return q_block <= 16 ? 1 : size == 2 && DP <= 32 ? 4 : 2; }
+// Tiles of 16 query rows of a wave: each key that is loaded serves them all, as long
+// as the registers hold them.  A training step of 40,000 points, 4 heads, 16 blocks,
+// with a bias: bf16 of 128 channels 2.27 ms with one tile, 2.40 with two (and one wave
+// a SIMD: 2.48 spilled for two; without a bias 1.51, 1.26 and 1.30), fp32 of 64 channels
+// 3.15 with two (spilled for two waves: 3.43 with one wave), 3.63 with one tile.
+constexpr int query_tiles(int size, int DP, int q_block, bool bias) {
+    return q_block <= 16 || (size == 2 && DP == 128 && bias) ? 1 : size == 2 && DP <= 32 ? 4 : 2;
+}
+constexpr int query_waves(int size, int DP, int RT) {
+    return DP * RT * size > 512 || DP * size == 512 || (size == 2 && DP * RT == 256) ? 1 : 2;
+}
 
 // Smallest value of the lanes of `todo` (32 lanes' bits; the wave's two halves
 // hold the same), on every lane.
@@ -65,10 +74,8 @@ constexpr int kWindow = 16;
 // list of them: tiles part, part + parts, ... of one head.
 template <typename T, int DP, int RT, bool kBias>
 __global__ __launch_bounds__(kWave)
-    __attribute__((amdgpu_waves_per_eu(DP * RT * sizeof(T) > 512 || DP * sizeof(T) == 512 ? 1 : 2))) void attend_dq_kernel(AttendArgs a,
-                                                                                                  AttendGrads gr,
-                                                                                                  int tiles,
-                                                                                                  int64_t items) {
+    __attribute__((amdgpu_waves_per_eu(query_waves(sizeof(T), DP, RT)))) void attend_dq_kernel(AttendArgs a, AttendGrads gr,
+                                                                                              int tiles, int64_t items) {
     constexpr int DS = DP / 32, DT = DP / 16, KT = kStep / 16, E = sizeof(T);
     constexpr int LD = turned_stride<T>(DP);
     constexpr int kPairs = (RT + 1) / 2, kQueries = 32 * kPairs;  // row tiles in twos
@@ -810,8 +817,8 @@ hipError_t launch_dkv(const AttendArgs& a, const AttendGrads& g, hipStream_t str
 
 template <typename T, int DP, bool kBias>
 hipError_t launch_pair(const AttendArgs& a, const AttendGrads& g, hipStream_t stream) {
-    hipError_t e = a.q_block <= 16 ? launch_dq<T, DP, query_tiles(sizeof(T), DP, 16), kBias>(a, g, stream)
-                                   : launch_dq<T, DP, query_tiles(sizeof(T), DP, 17), kBias>(a, g, stream);
+    hipError_t e = a.q_block <= 16 ? launch_dq<T, DP, query_tiles(sizeof(T), DP, 16, kBias), kBias>(a, g, stream)
+                                   : launch_dq<T, DP, query_tiles(sizeof(T), DP, 17, kBias), kBias>(a, g, stream);
     if (e != hipSuccess) return e;
     if constexpr (kBias) {
         const int bins = a.axes * a.buckets;
@@ -835,7 +842,7 @@ hipError_t launch_type(const AttendArgs& a, const AttendGrads& g, hipStream_t st
 }  // namespace
 
 int attend_table_parts(const AttendArgs& a, bool bf16) {
-    const int rows = 16 * query_tiles(bf16 ? 2 : 4, a.D <= 32 ? 32 : a.D <= 64 ? 64 : 128, a.q_block);
+    const int rows = 16 * query_tiles(bf16 ? 2 : 4, a.D <= 32 ? 32 : a.D <= 64 ? 64 : 128, a.q_block, true);
     const int64_t tiles = static_cast<int64_t>(a.groups) * ((a.q_block + rows - 1) / rows);
     const int64_t most = std::max(1, kTableWaves / a.heads);
     const int64_t each = std::max<int64_t>(1, (tiles + most - 1) / most);  // tiles of a wave
