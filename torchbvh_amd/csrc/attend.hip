@@ -29,6 +29,17 @@ constexpr int forward_waves(int DP, int RT, int W, bool bias) {
 // A wave holds its queries and sums in registers, takes 32 keys a step straight
 // into the first product's fragments, and turns the values' rows through LDS.
 // The next step's keys and values are loaded while this one's are used.
+//
+// Every key that is loaded serves RT * 16 rows: 262,144 points, 16 blocks of 64, 8
+// heads of 64 channels, bf16 take 850 us (550 GFLOP: 650 TFLOP/s; loads from the
+// caches 15 TB/s), where tiles of 32 rows took 1529 against 1110 for 64 at the
+// time.  With 242 registers two waves share a SIMD: the products take 0.25 ms of its
+// cycles, the vector instructions (the softmax, one exponential a score) 0.35 ms, and
+// two waves overlap these and the loads only in part.  Locality of the choice does not
+// count (the same blocks for all rows: no faster).  With a bias (16 clouds of 10,000
+// points, 8 blocks, 4 heads of 32 channels, two axes: 202 us) the table's lookups in
+// LDS and their adds, two a score, take over.  fp32's products run at an eighth of the
+// rate and need 64 channels a tile at most (see launch_rows).
 template <typename T, int DP, int RT, int W, bool kBias, bool kExact>
 __global__ __launch_bounds__(kWave* W) __attribute__((amdgpu_waves_per_eu(forward_waves<T>(DP, RT, W, kBias || kExact)))) void attend_kernel(AttendArgs a, int tiles, int64_t items) {
     constexpr int DS = DP / 32, DT = DP / 16, KT = kChunk / 16, E = sizeof(T);
@@ -430,7 +441,9 @@ hipError_t launch(const AttendArgs& a, hipStream_t stream) {
 
 // Row tiles: 16 rows where a block has no more, else 64, or 32 where the
 // accumulators of 64 would not fit the registers (fp32, more than 64
-// channels).  Waves per tile: enough that a call of few tiles covers the chip.
+// channels).  Waves per tile: enough that a call of few tiles covers the chip; a probe
+// of 16 blocks, 8 heads of 64 channels, takes 9.9 us so, of which two thirds are the
+// launch and two dependent loads before the first product.
 template <typename T, int DP>
 hipError_t launch_rows(const AttendArgs& a, hipStream_t stream) {
     constexpr int kWide = sizeof(T) == 2 && DP <= 64 ? 4 : 2;

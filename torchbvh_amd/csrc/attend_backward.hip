@@ -16,9 +16,15 @@ namespace {
 constexpr int kStep = 32;  // rows of the other side per step
 
 // Waves of the query-side kernel with a bias, over all heads: each takes many tiles
-// of one head, so that few parts of the table's gradient are left to add up.
+// of one head, so that few parts of the table's gradient are left to add up, and all
+// run at once, two a SIMD (a training step over 77,000 points: 2.21 ms, with 4096 waves
+// 2.42, with 8192 2.31; over 37,000 in fp32: 0.93, 1.03, 0.95).
 constexpr int kTableWaves = 2048;
 
+// Key tiles up to this many waves are split between four waves each: blocks are chosen
+// unequally often, and a wave alone with a long run keeps the launch waiting (77,000
+// points, 8 heads, 16 blocks: 749 us, with one wave a tile 862).  Beyond, the
+// tiles themselves even that out.
 constexpr int64_t kSplitWaves = 1 << 16;
 
 // Tiles of 16 query rows of a wave: each key that is loaded serves them all, as long
@@ -66,12 +72,19 @@ __device__ __forceinline__ Vec8<T> units(const int* cells, int g, int at) {
 // 16 cells of either side, the 16 x 16 sums G = sum_ij e(cq_i) ds_ij e(ck_j)^T are
 // two more products, and only G's 256 entries are added in LDS, four a lane, instead
 // of the step's every ds (adding each one took 193 cycles a wave instruction as an
-// LDS float atomic, 10.5 of 12 ms of a training step over 80,000 points).  Cells of a
+// LDS float atomic, 10.5 of 12 ms of a training step over 77,000 points).  Cells of a
 // block of neighbours mostly fit one window; more windows are taken as needed.
 constexpr int kWindow = 16;
 
 // One wave per (tile of RT * 16 rows of a row block, head), or, with a bias, per
 // list of them: tiles part, part + parts, ... of one head.
+//
+// 77,000 points in 8 clouds, 16 blocks of 64, 8 heads of 32 channels, bf16, three axes:
+// 1030 us.  The vector instructions issue in half of the cycles (a lookup and an add a
+// score and axis, the exponential, the unit vectors, the joins of ds and its rest);
+// the table's gradient is 30 % of the time; two waves a SIMD (254 registers) leave a
+// fifth of it waiting for LDS and loads.  fp32 (37,000 points, 4 heads of 24 channels):
+// 405 us, half of its cycles in the products, of which the unit vectors' are a third.
 template <typename T, int DP, int RT, bool kBias>
 __global__ __launch_bounds__(kWave)
     __attribute__((amdgpu_waves_per_eu(query_waves(sizeof(T), DP, RT)))) void attend_dq_kernel(AttendArgs a, AttendGrads gr,
@@ -298,8 +311,9 @@ __global__ __launch_bounds__(kWave)
 #pragma unroll
                                 for (int rt = 0; rt < RT; ++rt) ds[kt][rt][r] = 0.0f;
                 }
-                // ds is rounded to T for the product with k; the table's sums, in which the
-                // terms of a row cancel, also take what that leaves off.
+                // ds is rounded to T once for the product with k, which adds an error as large
+                // as dq's own rounding; the table's sums, in which the terms of a row cancel, also
+                // take what that leaves off.
                 Vec8<T> df[RT], dl[RT];
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) {
@@ -425,6 +439,12 @@ constexpr int key_tiles(int DP) { return sizeof(T) == 4 && DP == 128 ? 1 : 2; }
 // blocks of whole steps (kWhole) a step's rows are neighbours in one row block;
 // otherwise the blocks' rows are strung together and each lane finds its own.
 // W waves take every W-th step, and their sums are added in order.
+//
+// Keys and sums stay in registers, 32 keys of each head: the rows are read again by
+// every key block that they chose, out of the L2 (77,000 points as above: 750 us, the
+// vector instructions and LDS's turned reads of q and grad each half of the cycles; 64
+// keys a wave spilled and were slower).  A row's weights p and its ds are rounded to T
+// once for their products.
 template <typename T, int DP, int W, bool kBias, bool kWhole>
 __global__ __launch_bounds__(kWave* W)
     __attribute__((amdgpu_waves_per_eu(DP * sizeof(T) <= 128 ? 2 : 1))) void attend_dkv_kernel(AttendArgs a,

@@ -10,6 +10,13 @@
 // shape around the two sums per channel.  All sums are fp32 in a fixed order;
 // squares are summed around means (of eight rows, then of a thread's, then joined
 // by n, mean and squares), so a large mean costs no digits.
+//
+// Memory bounds all of it once the values outgrow the caches: what a cloud-wide sum
+// decides can only be applied in a second read.  One million rows of 256 channels
+// in bf16 (silu): stats 126 us (4.3 TB/s), join 11, apply 201 (5.3 TB/s), sums
+// 245 (4.4 TB/s), dx 321 (5.0 TB/s), 875 in all, against 5.2 TB/s for a large copy.
+// In the caches' reach (552,000 rows of 88 channels, gelu) the activation's
+// some twenty instructions a value count as much: apply 45, sums 66, dx 78 us.
 #include "norm.hpp"
 
 namespace tbvh {
@@ -433,7 +440,8 @@ __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(4))) voi
 }
 
 // One work-group per (group, cloud) whose values all fit its registers: mean, then
-// squares around it, then y, in one launch and one read.
+// squares around it, then y, in one launch and one read (1,000 rows of 64 channels: 7.6
+// us, the call 20.6, with the three launches 26).
 constexpr int kSmallThreads = 1024, kSmallVectors = 8;
 
 __device__ __forceinline__ float small_sum(float x, float* s_sum) {
