@@ -66,8 +66,8 @@ def _require(op: str, holds: bool, message: str) -> None:
 
 def block_layout(source, block_size: int = 64, *, device=None) -> BlockLayout:
     """The layout of a handle's points, of ``(B, N)`` equal clouds, or of packed
-    clouds given as ``(B + 1,)`` int64 CUDA offsets (read back to the host
-    once)."""
+    clouds given as ``(B + 1,)`` int64 CUDA offsets (which the host reads
+    back)."""
     op = "block_layout"
     _require(op, isinstance(block_size, int) and 1 <= block_size <= MAX_BLOCK, f"block_size must be 1 to {MAX_BLOCK}")
     if isinstance(source, RaggedBVHHandle):
