@@ -12,7 +12,8 @@ constexpr int kChunk = 32;  // keys per step of the running softmax
 // most steps need neither the maximum across lanes nor new sums.
 constexpr float kSlack = 8.0f;
 
-// Waves per SIMD that the registers are kept to (without spills).
+// Waves per SIMD that the registers are kept to (without spills, but for nine registers
+// of fp32 at 64 channels in tiles of 16 rows, where a wave less costs as much).
 template <typename T>
 constexpr int forward_waves(int DP, int RT, int W, bool bias) {
     const int words = DP * RT * static_cast<int>(sizeof(T));
@@ -107,12 +108,16 @@ __global__ __launch_bounds__(kWave* W) __attribute__((amdgpu_waves_per_eu(forwar
     }
 
     f32x4 acc[RT][DT], sums[RT];
-    // Weights are exp2(score - ref); a score that exceeds ref by over `limit` moves it.
-    float ref[RT], limit[RT], sum[RT];
+    // Weights are exp2(score - ref); a score that exceeds ref by `limit` or more moves it.
+    // Both as the integers that they are in memory: floats from 0 on are in the integers'
+    // order and negative ones below them, so one comparison tells, in a third of the
+    // instructions that maxima of floats (which quiet NaNs first) take.
+    float ref[RT], sum[RT];
+    int limit[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         ref[rt] = 0.0f;
-        limit[rt] = -INFINITY;  // no score yet: the first one sets it
+        limit[rt] = INT32_MIN;  // no score yet: the first one sets it
         sum[rt] = 0.0f;
         sums[rt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -227,26 +232,30 @@ __global__ __launch_bounds__(kWave* W) __attribute__((amdgpu_waves_per_eu(forwar
 #pragma unroll
                         for (int rt = 0; rt < RT; ++rt) st[kt][rt][r] = -INFINITY;
         }
-        float most[RT];
         bool above = false;
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-            float m = fmaxf(fmaxf(st[0][rt][0], st[0][rt][1]), fmaxf(st[0][rt][2], st[0][rt][3]));
+            int m = INT32_MIN;
 #pragma unroll
-            for (int kt = 1; kt < KT; ++kt)
-                m = fmaxf(fmaxf(fmaxf(m, st[kt][rt][0]), fmaxf(st[kt][rt][1], st[kt][rt][2])), st[kt][rt][3]);
-            most[rt] = m;
-            above |= m > limit[rt];
+            for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) m = max(m, __float_as_int(st[kt][rt][r]));
+            above |= m >= limit[rt];
         }
         if (__any(above)) {
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
                 // The largest score so far, and how far the reference follows: rows that
                 // have met no score above -inf keep a reference of 0 and weights of 0.
-                const float m = across_groups_max(most[rt]);
-                const bool first = limit[rt] < 0.0f;
+                float m = -INFINITY;
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) m = fmaxf(m, st[kt][rt][r]);
+                m = across_groups_max(m);
+                const bool first = limit[rt] < 0;
                 const float up = first ? (m == -INFINITY ? 0.0f : m) : fmaxf(m, 0.0f);
-                if (m != -INFINITY) limit[rt] = kSlack;
+                if (m != -INFINITY) limit[rt] = __float_as_int(kSlack);
                 // The sums are 0 before the first score, which may be far below 0.
                 const float keep = first ? 0.0f : __builtin_amdgcn_exp2f(-up);
                 ref[rt] += up;
@@ -350,7 +359,7 @@ __global__ __launch_bounds__(kWave* W) __attribute__((amdgpu_waves_per_eu(forwar
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             float* p = s_part + wave * kPer + rt * (DT * 4 + 2) * kWave + lane;
-            p[0] = limit[rt] < 0.0f ? -INFINITY : ref[rt];
+            p[0] = limit[rt] < 0 ? -INFINITY : ref[rt];
             p[kWave] = sum[rt];
 #pragma unroll
             for (int t = 0; t < DT; ++t)
