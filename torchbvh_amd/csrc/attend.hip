@@ -22,6 +22,14 @@ constexpr int forward_waves(int DP, int RT, int W, bool bias) {
     return most - (tight && most > 1 ? 1 : 0);
 }
 
+// Cells that unit vectors tell apart, and whether a tile may take the bias as products.
+constexpr int kWindow = 16;
+template <typename T, int RT>
+__host__ __device__ __forceinline__ bool by_products(const AttendArgs& a) {
+    return sizeof(T) == 2 && RT > 1 && a.share == 1;
+}
+__host__ __device__ __forceinline__ int table_words(int reach) { return 2 * (reach + kWindow) + 1; }
+
 // One work-group of W waves per (row block, key head, tile of RT * 16 rows of
 // the block's queries times the heads that share the key head); wave w takes
 // every W-th chosen block, and the waves' parts are joined at the end.
@@ -61,8 +69,13 @@ __global__ __launch_bounds__(kWave* W) __attribute__((amdgpu_waves_per_eu(forwar
     if (tile * RT * 16 >= rows) return;
 
     T* s_v = reinterpret_cast<T*>(s_raw) + wave * kChunk * LDV;
-    int* s_cell = reinterpret_cast<int*>(reinterpret_cast<T*>(s_raw) + W * kChunk * LDV) + wave * 3 * kChunk;
-    float* s_bias = reinterpret_cast<float*>(reinterpret_cast<T*>(s_raw) + W * kChunk * LDV) + W * 3 * kChunk;
+    // Unit vectors of the rows' cells, for a pair of axes and a row tile a fragment.
+    const int axis_pairs = kBias && by_products<T, RT>(a) ? (a.axes + 1) / 2 : 0;
+    Vec8<T>* s_units = reinterpret_cast<Vec8<T>*>(reinterpret_cast<T*>(s_raw) + W * kChunk * LDV) + wave * axis_pairs * RT * kWave;
+    int* s_cells = reinterpret_cast<int*>(reinterpret_cast<Vec8<T>*>(reinterpret_cast<T*>(s_raw) + W * kChunk * LDV) +
+                                          W * axis_pairs * RT * kWave);
+    int* s_cell = s_cells + wave * 3 * kChunk;
+    float* s_bias = reinterpret_cast<float*>(s_cells + W * 3 * kChunk);
     const int span = 2 * a.reach + 1, entries = a.axes * span, reach = 4 * a.reach;
     if constexpr (kBias) {
         const T* table = static_cast<const T*>(a.table);
@@ -71,8 +84,29 @@ __global__ __launch_bounds__(kWave* W) __attribute__((amdgpu_waves_per_eu(forwar
             const int b = min(max(a.map[e - axis * span], 0), a.buckets - 1);
             s_bias[i] = static_cast<float>(table[(axis * a.buckets + b) * a.heads + c * a.share + hs]) * kLog2e;
         }
-        __syncthreads();
     }
+    // (2 * axis_pairs, wide): the table at distances -(reach + kWindow) .. reach + kWindow,
+    // each with the next one's in the upper half of its word; 0 for an axis that is not there.
+    const int wide = table_words(a.reach);
+    uint32_t* s_pair = reinterpret_cast<uint32_t*>(s_bias + a.share * entries);
+    bool finite = true;
+    if constexpr (kBias && E == 2) {
+        const uint16_t* table = static_cast<const uint16_t*>(a.table);
+        for (int i = threadIdx.x; i < 2 * axis_pairs * wide; i += kWave * W) {
+            const int axis = i / wide, e = i - axis * wide - a.reach - kWindow;
+            uint32_t word = 0;
+            if (axis < a.axes) {
+                const auto at = [&](int distance) -> uint32_t {
+                    const int b = min(max(a.map[min(max(distance, -a.reach), a.reach) + a.reach], 0), a.buckets - 1);
+                    return table[(axis * a.buckets + b) * a.heads + c];
+                };
+                word = at(e) | at(e + 1) << 16;
+                finite &= (word & 0x7f80u) != 0x7f80u && (word & 0x7f800000u) != 0x7f800000u;
+            }
+            s_pair[i] = word;
+        }
+    }
+    if constexpr (kBias) finite = __syncthreads_and(finite);
 
     const float to_log2 = a.scale * kLog2e;
     Vec8<T> qf[RT][DS];
@@ -104,6 +138,35 @@ __global__ __launch_bounds__(kWave* W) __attribute__((amdgpu_waves_per_eu(forwar
             }
             close_from[x] = largest_lane(hi) - reach;
             close_span[x] = least_lane(lo) + reach - close_from[x];
+        }
+    }
+    // In bf16 the bias is mostly two more products (one for two axes): unit vectors of
+    // the rows' cells, of which kWindow neighbouring ones are told apart, times what the
+    // table gives a key at each of these.  The table's values are exact in bf16, one of
+    // them is multiplied by 1 and the others by 0, so nothing is rounded; a table that
+    // is not finite, rows further apart or several heads in a tile take the lookups.
+    bool quick = axis_pairs > 0 && finite;
+    int window[3] = {};
+    if constexpr (kBias && E == 2) {
+#pragma unroll
+        for (int x = 0; x < 3; ++x) {
+            const int most = close_from[x] + reach;
+            window[x] = close_from[x] + close_span[x] - reach;
+            quick = quick && most - window[x] < 4 * kWindow;
+        }
+        if (quick) {
+            for (int m = 0; m < axis_pairs; ++m) {
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    const int second = 2 * m + 1 < a.axes;  // of the pair
+                    const int cell = m == 0 ? (g < 2 ? qc[rt][0] - window[0] : qc[rt][1] - window[1]) : qc[rt][2] - window[2];
+                    const int slot = g < 2 || second ? cell / 4 - 8 * (g & 1) : -1;
+                    Vec8<T> u;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) u[j] = static_cast<T>(slot == j ? 1.0f : 0.0f);
+                    s_units[(m * RT + rt) * kWave + lane] = u;
+                }
+            }
         }
     }
 
@@ -188,13 +251,41 @@ __global__ __launch_bounds__(kWave* W) __attribute__((amdgpu_waves_per_eu(forwar
             }
         load_keys();
         // Scores less the reference, in powers of two.
+        if (kBias && E == 2 && quick) {
+            if constexpr (kBias && E == 2) {
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt)
+                for (int kt = 0; kt < KT; ++kt) {
+                    f32x4 bias[RT];
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
+                    for (int m = 0; m < 2; ++m) {
+                        if (m >= axis_pairs) continue;
+                        const int axis = 2 * m + (g >> 1), low = m == 0 ? (g < 2 ? window[0] : window[1]) : window[2];
+                        const int cell = s_cell[min(axis, a.axes - 1) * kChunk + 16 * kt + n];
+                        const uint32_t* at = s_pair + axis * wide + a.reach + kWindow + 8 * (g & 1) +
+                                             min(max(low - cell, -reach - 4 * kWindow), reach) / 4;
+                        const Vec8<T> of = __builtin_bit_cast(Vec8<T>, Words4{at[0], at[2], at[4], at[6]});
 #pragma unroll
-                for (int r = 0; r < 4; ++r) st[kt][rt][r] = __builtin_fmaf(st[kt][rt][r], to_log2, -ref[rt]);
-        if constexpr (kBias) {
+                        for (int rt = 0; rt < RT; ++rt)
+                            bias[rt] = mma(of, s_units[(m * RT + rt) * kWave + lane],
+                                           m == 0 ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : bias[rt]);
+                    }
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            st[kt][rt][r] = __builtin_fmaf(st[kt][rt][r], to_log2,
+                                                           __builtin_fmaf(bias[rt][r], kLog2e, -ref[rt]));
+                }
+            }
+        } else {
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) st[kt][rt][r] = __builtin_fmaf(st[kt][rt][r], to_log2, -ref[rt]);
+        }
+        if (kBias && !quick) {
 #pragma unroll
             for (int x = 0; x < 3; ++x) {
                 if (x >= a.axes) continue;
@@ -428,8 +519,10 @@ hipError_t launch(const AttendArgs& a, hipStream_t stream) {
     const int64_t items = static_cast<int64_t>(a.groups) * tiles * a.kv_heads;
     const unsigned grid = static_cast<unsigned>(xcd_grid(items));
     const size_t stage = static_cast<size_t>(W) * kChunk * turned_stride<T>(DP) * sizeof(T);
-    const size_t bias = static_cast<size_t>(W) * 3 * kChunk * sizeof(int) +
-                        static_cast<size_t>(a.share) * a.axes * (2 * a.reach + 1) * sizeof(float);
+    const size_t pairs = by_products<T, RT>(a) ? (a.axes + 1) / 2 : 0;
+    const size_t bias = static_cast<size_t>(W) * (3 * kChunk * sizeof(int) + pairs * RT * kWave * 8 * sizeof(T)) +
+                        static_cast<size_t>(a.share) * a.axes * (2 * a.reach + 1) * sizeof(float) +
+                        2 * pairs * table_words(a.reach) * sizeof(uint32_t);
     const size_t parts = W > 1 ? static_cast<size_t>(W) * RT * (DP / 16 * 4 + 2) * kWave * sizeof(float) : 0;
     const size_t lds = std::max(stage + (a.table != nullptr ? bias : 0), parts);
     const auto run = [&](auto kernel) {
