@@ -22,13 +22,11 @@ constexpr int forward_waves(int DP, int RT, int W, bool bias) {
     return most - (tight && most > 1 ? 1 : 0);
 }
 
-// Cells that unit vectors tell apart, and whether a tile may take the bias as products.
-constexpr int kWindow = 16;
+// Whether a tile may take the bias as products: its rows read one table.
 template <typename T, int RT>
 __host__ __device__ __forceinline__ bool by_products(const AttendArgs& a) {
     return sizeof(T) == 2 && RT > 1 && a.share == 1;
 }
-__host__ __device__ __forceinline__ int table_words(int reach) { return 2 * (reach + kWindow) + 1; }
 
 // One work-group of W waves per (row block, key head, tile of RT * 16 rows of
 // the block's queries times the heads that share the key head); wave w takes
@@ -85,28 +83,10 @@ __global__ __launch_bounds__(kWave* W) __attribute__((amdgpu_waves_per_eu(forwar
             s_bias[i] = static_cast<float>(table[(axis * a.buckets + b) * a.heads + c * a.share + hs]) * kLog2e;
         }
     }
-    // (2 * axis_pairs, wide): the table at distances -(reach + kWindow) .. reach + kWindow,
-    // each with the next one's in the upper half of its word; 0 for an axis that is not there.
-    const int wide = table_words(a.reach);
     uint32_t* s_pair = reinterpret_cast<uint32_t*>(s_bias + a.share * entries);
-    bool finite = true;
-    if constexpr (kBias && E == 2) {
-        const uint16_t* table = static_cast<const uint16_t*>(a.table);
-        for (int i = threadIdx.x; i < 2 * axis_pairs * wide; i += kWave * W) {
-            const int axis = i / wide, e = i - axis * wide - a.reach - kWindow;
-            uint32_t word = 0;
-            if (axis < a.axes) {
-                const auto at = [&](int distance) -> uint32_t {
-                    const int b = min(max(a.map[min(max(distance, -a.reach), a.reach) + a.reach], 0), a.buckets - 1);
-                    return table[(axis * a.buckets + b) * a.heads + c];
-                };
-                word = at(e) | at(e + 1) << 16;
-                finite &= (word & 0x7f80u) != 0x7f80u && (word & 0x7f800000u) != 0x7f800000u;
-            }
-            s_pair[i] = word;
-        }
-    }
-    if constexpr (kBias) finite = __syncthreads_and(finite);
+    bool small = true;
+    if constexpr (kBias && E == 2) small = fill_pairs(s_pair, a, c, axis_pairs, false, threadIdx.x, kWave * W);
+    if constexpr (kBias) small = __syncthreads_and(small);
 
     const float to_log2 = a.scale * kLog2e;
     Vec8<T> qf[RT][DS];
@@ -140,12 +120,8 @@ __global__ __launch_bounds__(kWave* W) __attribute__((amdgpu_waves_per_eu(forwar
             close_span[x] = least_lane(lo) + reach - close_from[x];
         }
     }
-    // In bf16 the bias is mostly two more products (one for two axes): unit vectors of
-    // the rows' cells, of which kWindow neighbouring ones are told apart, times what the
-    // table gives a key at each of these.  The table's values are exact in bf16, one of
-    // them is multiplied by 1 and the others by 0, so nothing is rounded; a table that
-    // is not finite, rows further apart or several heads in a tile take the lookups.
-    bool quick = axis_pairs > 0 && finite;
+    const float unscale = 1.0f / a.scale;
+    bool quick = axis_pairs > 0 && small && unscalable(a.scale);
     int window[3] = {};
     if constexpr (kBias && E == 2) {
 #pragma unroll
@@ -158,13 +134,8 @@ __global__ __launch_bounds__(kWave* W) __attribute__((amdgpu_waves_per_eu(forwar
             for (int m = 0; m < axis_pairs; ++m) {
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) {
-                    const int second = 2 * m + 1 < a.axes;  // of the pair
-                    const int cell = m == 0 ? (g < 2 ? qc[rt][0] - window[0] : qc[rt][1] - window[1]) : qc[rt][2] - window[2];
-                    const int slot = g < 2 || second ? cell / 4 - 8 * (g & 1) : -1;
-                    Vec8<T> u;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) u[j] = static_cast<T>(slot == j ? 1.0f : 0.0f);
-                    s_units[(m * RT + rt) * kWave + lane] = u;
+                    s_units[(m * RT + rt) * kWave + lane] = unit_slots<T>(
+                        m == 0 ? (g < 2 ? qc[rt][0] - window[0] : qc[rt][1] - window[1]) : qc[rt][2] - window[2], g);
                 }
             }
         }
@@ -244,47 +215,41 @@ __global__ __launch_bounds__(kWave* W) __attribute__((amdgpu_waves_per_eu(forwar
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                st[kt][rt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int s = 0; s < DS; ++s) st[kt][rt] = mma(kf[kt][s], qf[rt][s], st[kt][rt]);
-            }
-        load_keys();
-        // Scores less the reference, in powers of two.
-        if (kBias && E == 2 && quick) {
-            if constexpr (kBias && E == 2) {
+            for (int rt = 0; rt < RT; ++rt) st[kt][rt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if constexpr (kBias && E == 2) {
+            if (quick) {
 #pragma unroll
                 for (int kt = 0; kt < KT; ++kt) {
-                    f32x4 bias[RT];
 #pragma unroll
                     for (int m = 0; m < 2; ++m) {
                         if (m >= axis_pairs) continue;
                         const int axis = 2 * m + (g >> 1), low = m == 0 ? (g < 2 ? window[0] : window[1]) : window[2];
                         const int cell = s_cell[min(axis, a.axes - 1) * kChunk + 16 * kt + n];
-                        const uint32_t* at = s_pair + axis * wide + a.reach + kWindow + 8 * (g & 1) +
-                                             min(max(low - cell, -reach - 4 * kWindow), reach) / 4;
-                        const Vec8<T> of = __builtin_bit_cast(Vec8<T>, Words4{at[0], at[2], at[4], at[6]});
+                        const Vec8<T> of = pair_slots(s_pair, a, axis, g, low - cell);
 #pragma unroll
                         for (int rt = 0; rt < RT; ++rt)
-                            bias[rt] = mma(of, s_units[(m * RT + rt) * kWave + lane],
-                                           m == 0 ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : bias[rt]);
+                            st[kt][rt] = mma(of, s_units[(m * RT + rt) * kWave + lane], st[kt][rt]);
                     }
 #pragma unroll
-                    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            st[kt][rt][r] = __builtin_fmaf(st[kt][rt][r], to_log2,
-                                                           __builtin_fmaf(bias[rt][r], kLog2e, -ref[rt]));
+                    for (int rt = 0; rt < RT; ++rt) st[kt][rt] *= unscale;
                 }
             }
-        } else {
-#pragma unroll
-            for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) st[kt][rt][r] = __builtin_fmaf(st[kt][rt][r], to_log2, -ref[rt]);
         }
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+                for (int s = 0; s < DS; ++s) st[kt][rt] = mma(kf[kt][s], qf[rt][s], st[kt][rt]);
+            }
+        load_keys();
+        // Scores less the reference, in powers of two.
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) st[kt][rt][r] = __builtin_fmaf(st[kt][rt][r], to_log2, -ref[rt]);
         if (kBias && !quick) {
 #pragma unroll
             for (int x = 0; x < 3; ++x) {

@@ -229,6 +229,59 @@ __device__ __forceinline__ int cell_bytes(int cell) { return min(max(cell, -kFar
 // The distance of two such cells, clamped to [-reach, reach] (in bytes).
 __device__ __forceinline__ int cell_distance(int a, int b, int reach) { return min(max(a - b, -reach), reach); }
 
+// In bf16 the bias is mostly a product, or two for three axes: unit vectors of one
+// side's cells, of which kWindow neighbouring ones on an axis are told apart, times
+// what the table gives the other side at each of these.  The table's values are exact
+// in bf16 and one of them is multiplied by 1, the others by 0, so nothing is rounded.
+// Tables with values of 2^64 and more (or none: infinities), a scale far from 1 and
+// cells further apart take a lookup for every score.
+// The sums start from bias / scale, the other product follows and the scale comes last.
+constexpr int kWindow = 16;
+__device__ __forceinline__ bool unscalable(float scale) { return fabsf(scale) > 1e-12f && fabsf(scale) < 1e12f; }
+__host__ __device__ __forceinline__ int table_words(int reach) { return 2 * (reach + kWindow) + 1; }
+
+// A head's tables of bf16 for it, (2 * axis_pairs, table_words): entry e is distance
+// e - reach - kWindow (or its negative), with the next entry in the upper half of its
+// word; 0 for an axis that is not there.  Says whether this thread's were
+// all small enough to be divided by the scale.
+__device__ __forceinline__ bool fill_pairs(uint32_t* to, const AttendArgs& a, int head, int axis_pairs, bool negative,
+                                           int thread, int threads) {
+    const uint16_t* table = static_cast<const uint16_t*>(a.table);
+    const int wide = table_words(a.reach);
+    bool small = true;
+    for (int i = thread; i < 2 * axis_pairs * wide; i += threads) {
+        const int axis = i / wide, e = i - axis * wide - a.reach - kWindow;
+        uint32_t word = 0;
+        if (axis < a.axes) {
+            const auto at = [&](int distance) -> uint32_t {
+                const int d = min(max(negative ? -distance : distance, -a.reach), a.reach);
+                const int b = min(max(a.map[d + a.reach], 0), a.buckets - 1);
+                return table[(axis * a.buckets + b) * a.heads + head];
+            };
+            word = at(e) | at(e + 1) << 16;
+            small &= (word & 0x7f80u) < 0x5f80u && (word & 0x7f800000u) < 0x5f800000u;  // 2^64
+        }
+        to[i] = word;
+    }
+    return small;
+}
+// What lane group g takes of them: slots 8 (g % 2) .. + 7 of an axis whose distance in
+// bytes at slot 0 is `from`.
+__device__ __forceinline__ bf16x8 pair_slots(const uint32_t* pairs, const AttendArgs& a, int axis, int g, int from) {
+    const uint32_t* at = pairs + axis * table_words(a.reach) + a.reach + kWindow + 8 * (g & 1) +
+                         min(max(from, -4 * (a.reach + kWindow)), 4 * a.reach) / 4;
+    return __builtin_bit_cast(bf16x8, Words4{at[0], at[2], at[4], at[6]});
+}
+// A unit vector's slots 8 (g % 2) .. + 7, of a cell `apart` bytes past slot 0.
+template <typename T>
+__device__ __forceinline__ Vec8<T> unit_slots(int apart, int g) {
+    const int slot = apart / 4 - 8 * (g & 1);
+    Vec8<T> u;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) u[j] = static_cast<T>(slot == j ? 1.0f : 0.0f);
+    return u;
+}
+
 // Least and largest value of a wave's lanes, in scalar registers.
 __device__ __forceinline__ int least_lane(int v) {
     v = min(v, __builtin_amdgcn_update_dpp(v, v, 0x128, 0xf, 0xf, false));  // rows of 16 rotated by 8, 4, 2, 1

@@ -74,8 +74,6 @@ __device__ __forceinline__ Vec8<T> units(const int* cells, int g, int at) {
 // of the step's every ds (adding each one took 193 cycles a wave instruction as an
 // LDS float atomic, 10.5 of 12 ms of a training step over 77,000 points).  Cells of a
 // block of neighbours mostly fit one window; more windows are taken as needed.
-constexpr int kWindow = 16;
-
 // One wave per (tile of RT * 16 rows of a row block, head), or, with a bias, per
 // list of them: tiles part, part + parts, ... of one head.
 //
@@ -104,12 +102,21 @@ __global__ __launch_bounds__(kWave)
     int* s_cell = reinterpret_cast<int*>(s_k + kStep * LD);  // (3, 32) of the keys
     int* s_query = s_cell + 3 * kStep;                       // (3, kQueries) of the queries
     const int span = 2 * a.reach + 1, entries = a.axes * span, bins = a.axes * a.buckets, reach = 4 * a.reach;
-    Vec8<T>* s_units = reinterpret_cast<Vec8<T>*>(s_query + 3 * kQueries);  // (3, kPairs, 64) of the queries' first window
+    // Unit vectors of the queries' cells in their first window: in bf16 a row of kWindow
+    // a query and axis, read along the slots for the bias and turned for the table's
+    // gradient; in fp32 (3, kPairs, 64) fragments of the latter.
+    Vec8<T>* s_units = reinterpret_cast<Vec8<T>*>(s_query + 3 * kQueries);
+    T* s_rows = reinterpret_cast<T*>(s_units);
     float* s_bias = reinterpret_cast<float*>(s_units + 3 * kPairs * kWave);
+    const int axis_pairs = kBias && E == 2 ? (a.axes + 1) / 2 : 0;
     // Sums by distance, -(reach + 31) to reach + 31, a copy for each g: the lanes of
     // one copy always add at different distances.
     const int wide = 2 * (a.reach + 2 * kWindow) - 1;
     float* s_sum = s_bias + entries;  // (axes, 4, wide)
+    uint32_t* s_pair = reinterpret_cast<uint32_t*>(s_sum + a.axes * 4 * wide);
+    const float unscale = 1.0f / a.scale;
+    bool small = false;
+    if constexpr (kBias && E == 2) small = __all(fill_pairs(s_pair, a, h, axis_pairs, false, lane, kWave));
     if constexpr (kBias) {
         const T* table = static_cast<const T*>(a.table);
         for (int e = lane; e < entries; e += kWave) {
@@ -139,6 +146,7 @@ __global__ __launch_bounds__(kWave)
         Vec8<T> qf[RT][DS], gf[RT][DS];
         float lse[RT], delta[RT];
         int q_least[3] = {}, q_most[3] = {};  // cells of the tile's queries
+        bool quick = small && unscalable(a.scale);
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             const bool real = rt * 16 + n < here;
@@ -182,10 +190,19 @@ __global__ __launch_bounds__(kWave)
                 const int q = s_query[x * kQueries + (lane & (kQueries - 1))];
                 q_least[x] = least_lane(q);
                 q_most[x] = largest_lane(q);
+                quick = quick && q_most[x] - q_least[x] < 4 * kWindow;
+                if constexpr (E == 2) {
+                    T* row = s_rows + (x * kQueries + (lane & (kQueries - 1))) * kWindow;
+                    *reinterpret_cast<Vec8<T>*>(row) = unit_slots<T>(q - q_least[x], 0);
+                    *reinterpret_cast<Vec8<T>*>(row + 8) = unit_slots<T>(q - q_least[x], 1);
+                } else {
 #pragma unroll
-                for (int p = 0; p < kPairs; ++p)
-                    s_units[(x * kPairs + p) * kWave + lane] = units<T>(s_query + x * kQueries + 32 * p, g, q_least[x] + 4 * n);
+                    for (int p = 0; p < kPairs; ++p)
+                        s_units[(x * kPairs + p) * kWave + lane] =
+                            units<T>(s_query + x * kQueries + 32 * p, g, q_least[x] + 4 * n);
+                }
             }
+            wave_sync();
         }
         f32x4 acc[RT][DT];
 #pragma unroll
@@ -242,8 +259,34 @@ __global__ __launch_bounds__(kWave)
 #pragma unroll
                 for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) st[kt][rt] = ds[kt][rt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                if constexpr (kBias && E == 2) {
+                    if (quick) {
+#pragma unroll
+                        for (int kt = 0; kt < KT; ++kt) {
+#pragma unroll
+                            for (int m = 0; m < 2; ++m) {
+                                if (m >= axis_pairs) continue;
+                                const int axis = 2 * m + (g >> 1), there = min(axis, a.axes - 1);
+                                const int low = m == 0 ? (g < 2 ? q_least[0] : q_least[1]) : q_least[2];
+                                const Vec8<T> of =
+                                    pair_slots(s_pair, a, axis, g, low - s_cell[there * kStep + 16 * kt + n]);
+#pragma unroll
+                                for (int rt = 0; rt < RT; ++rt) {
+                                    const Vec8<T> u = *reinterpret_cast<const Vec8<T>*>(
+                                        s_rows + (there * kQueries + 16 * rt + n) * kWindow + 8 * (g & 1));
+                                    st[kt][rt] = mma(of, u, st[kt][rt]);
+                                }
+                            }
+#pragma unroll
+                            for (int rt = 0; rt < RT; ++rt) st[kt][rt] *= unscale;
+                        }
+                    }
+                }
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
                     for (int rt = 0; rt < RT; ++rt) {
-                        st[kt][rt] = ds[kt][rt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                         for (int s = 0; s < DS; ++s) {
                             st[kt][rt] = mma(kf[kt][s], qf[rt][s], st[kt][rt]);
@@ -263,7 +306,7 @@ __global__ __launch_bounds__(kWave)
                     for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
                         for (int r = 0; r < 4; ++r) st[kt][rt][r] = __builtin_fmaf(st[kt][rt][r], to_log2, -lse[rt]);
-                if constexpr (kBias) {
+                if (kBias && !quick) {
 #pragma unroll
                     for (int x = 0; x < 3; ++x) {
                         if (x >= a.axes) continue;
@@ -350,9 +393,14 @@ __global__ __launch_bounds__(kWave)
                                 f32x4 sums = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                                 for (int p = 0; p < kPairs; ++p) {
-                                    const Vec8<T> qu = q_low == q_least[x]
-                                                           ? s_units[(x * kPairs + p) * kWave + lane]
-                                                           : units<T>(s_query + x * kQueries + 32 * p, g, q_low + 4 * n);
+                                    Vec8<T> qu;
+                                    if (q_low != q_least[x]) {
+                                        qu = units<T>(s_query + x * kQueries + 32 * p, g, q_low + 4 * n);
+                                    } else if constexpr (E == 2) {
+                                        qu = load_turned<T, kWindow>(s_rows + (x * kQueries + 32 * p) * kWindow, 0, n, g);
+                                    } else {
+                                        qu = s_units[(x * kPairs + p) * kWave + lane];
+                                    }
                                     sums = mma(qu, part[p], sums);
                                     if constexpr (E == 2) sums = mma(qu, part_left[p], sums);
                                 }
@@ -802,7 +850,8 @@ hipError_t launch_dq(const AttendArgs& a, const AttendGrads& g, hipStream_t stre
     const size_t lds = kStep * turned_stride<T>(DP) * sizeof(T) + 3 * (kStep + 32 * ((RT + 1) / 2)) * sizeof(int) +
                        (kBias ? (entries + static_cast<size_t>(a.axes) * 4 * (2 * (a.reach + 2 * kWindow) - 1)) *
                                         sizeof(float) +
-                                    3 * ((RT + 1) / 2) * kWave * 8 * sizeof(T)
+                                    3 * ((RT + 1) / 2) * kWave * 8 * sizeof(T) +
+                                    (sizeof(T) == 2 ? (a.axes + 1) / 2 * 2 * table_words(a.reach) * sizeof(uint32_t) : 0)
                               : 0);
     const auto kernel = attend_dq_kernel<T, DP, RT, kBias>;
     const hipError_t e = allow_lds(kernel, lds);
