@@ -174,3 +174,62 @@ def test_roundings_in_bfloat16(axes):
     for name, (value, _) in want.items():
         off = ((got[name].detach().cpu().double() - value).norm() / value.norm()).item()
         assert off <= (one if name in ("out", "dtable") else 1.5 * 2**0.5 * one), (name, off)
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(2, 2), (8, 1), (18, 1)])
+@pytest.mark.parametrize("scale", [None, 0.0, -2.0, 1e-20])
+@pytest.mark.parametrize("spread", [3, 9, 400])
+def test_biases_by_products_and_by_lookups(heads, kv_heads, scale, spread):
+    """bf16: cells within 16 of each other and further apart, scales that nothing is
+    divided by, heads that share many tables."""
+    kind, layout = torch.bfloat16, _layout([130, 50], 64)
+    q, up = (_normal(i, kind, 180, heads, 16) for i in range(2))
+    k, v = (_normal(i, kind, 180, kv_heads, 16) for i in (2, 3))
+    cells = [torch.randint(-spread, spread + 1, (180, 3), dtype=torch.int32, device="cuda") for _ in range(2)]
+    cells[0][64:128] //= 4
+    bias = (_normal(5, kind, 3, 9, heads), tb.relative_buckets(5, 12), *cells)
+    selected = torch.tensor([[0, 1, 2], [2, 0, -1], [1, 1, 0], [3, -1, -1]], dtype=torch.int32, device="cuda")
+    got = _grads(q, k, v, up, selected, layout, layout, scale, tb.RelativeBias(*bias))
+    times = ref.multiplicity(selected, layout.starts.tolist(), layout.starts.tolist())
+    ref.within(got, ref.attention(q, k, v, times, 0.25 if scale is None else scale, bias, up))
+
+
+@pytest.mark.parametrize("value", [float("-inf"), -1e30, 1e25])
+def test_tables_that_are_not_small(value):
+    """A bucket that nothing may be chosen from, and one that outweighs everything."""
+    kind, layout = torch.bfloat16, _layout([128], 64)
+    q, k, v, up = (_normal(i, kind, 128, 2, 32) for i in range(4))
+    cells = torch.randint(-4, 5, (128, 2), dtype=torch.int32, device="cuda")
+    table = _normal(5, kind, 2, 9, 2)
+    table[0, 6] = value
+    bias = (table, tb.relative_buckets(5, 6), cells, cells)
+    selected = torch.tensor([[0, 1], [1, 0]], dtype=torch.int32, device="cuda")
+    got = _grads(q, k, v, up, selected, layout, layout, None, tb.RelativeBias(*bias))
+    big = torch.tensor(value, dtype=kind).double().item()
+    s = torch.einsum("ihd,jhd->hij", q.cpu().double(), k.cpu().double()) * 32**-0.5
+    which = bias[1].cpu()[(cells[:, None] - cells[None]).cpu().clamp(-6, 6) + 6].long()
+    for axis in range(2):
+        s = s + table.cpu().double()[axis][which[..., axis]].permute(2, 0, 1)
+    p = torch.softmax(s, -1)
+    want = torch.einsum("hij,jhd->ihd", p, v.cpu().double())
+    assert abs(big) > 2.0**64
+    # Where the table outweighs, scores differ by less than its own digits: any of them may win.
+    if value < 0:
+        assert ((got["out"].cpu().double() - want).abs() <= 2.0**-7 * 4).all()
+        assert all(torch.isfinite(t).all() for t in got.values())
+    else:
+        assert torch.isfinite(got["out"]).all()
+
+
+@pytest.mark.parametrize("axes,reach,D", [(1, 2047, 128), (3, 682, 32), (3, 682, 128)])
+def test_tables_as_large_as_they_may_be(axes, reach, D):
+    kind, layout = torch.bfloat16, _layout([150], 64)
+    q, k, v, up = (_normal(i, kind, 150, 2, D) for i in range(4))
+    cells = torch.randint(-reach, reach, (150, axes), dtype=torch.int32, device="cuda")
+    cells[:70] = cells[:70] % 9
+    sizes = {1: 128, 3: 43}[axes]
+    bias = (_normal(5, kind, axes, 2 * sizes - 1, 2), tb.relative_buckets(sizes, reach), cells, cells)
+    selected = torch.tensor([[0, 1], [2, 0], [1, 2]], dtype=torch.int32, device="cuda")
+    got = _grads(q, k, v, up, selected, layout, layout, None, tb.RelativeBias(*bias))
+    times = ref.multiplicity(selected, layout.starts.tolist(), layout.starts.tolist())
+    ref.within(got, ref.attention(q, k, v, times, D**-0.5, bias, up))

@@ -482,6 +482,12 @@ __global__ __launch_bounds__(kWave) void table_sum_kernel(const float* __restric
 template <typename T>
 constexpr int key_tiles(int DP) { return sizeof(T) == 4 && DP == 128 ? 1 : 2; }
 
+// Products that the bias takes there: of more heads the LDS might not hold the tables.
+template <typename T>
+__host__ __device__ __forceinline__ int key_axis_pairs(const AttendArgs& a) {
+    return sizeof(T) == 2 && a.share <= 8 ? (a.axes + 1) / 2 : 0;
+}
+
 // One wave per (KT * 16 rows of a key block, key head): the rows of every row block
 // that chose it, for every head that shares the key head, 32 at a time.  With
 // blocks of whole steps (kWhole) a step's rows are neighbours in one row block;
@@ -495,7 +501,7 @@ constexpr int key_tiles(int DP) { return sizeof(T) == 4 && DP == 128 ? 1 : 2; }
 // once for their products.
 template <typename T, int DP, int W, bool kBias, bool kWhole>
 __global__ __launch_bounds__(kWave* W)
-    __attribute__((amdgpu_waves_per_eu(DP * sizeof(T) <= 128 ? 2 : 1))) void attend_dkv_kernel(AttendArgs a,
+    __attribute__((amdgpu_waves_per_eu(DP * sizeof(T) <= 64 && kWhole ? 3 : DP * sizeof(T) <= 128 ? 2 : 1))) void attend_dkv_kernel(AttendArgs a,
                                                                                               AttendGrads gr, int tiles,
                                                                                               int64_t items) {
     constexpr int DS = DP / 32, DT = DP / 16, KT = key_tiles<T>(DP), RT = kStep / 16, E = sizeof(T);
@@ -516,7 +522,7 @@ __global__ __launch_bounds__(kWave* W)
     T* s_q = reinterpret_cast<T*>(reinterpret_cast<char*>(s_raw) + wave * kStage);
     T* s_g = s_q + kStep * LD;
     int* s_cell = reinterpret_cast<int*>(s_g + kStep * LD);  // (3, 32)
-    int* s_head = s_cell + 3 * kStep;                        // byte offset of the row's head's table
+    int* s_head = s_cell + 3 * kStep;                        // the row's head of those that share; in fp32 its table's byte
     float* s_lse = reinterpret_cast<float*>(s_head + kStep);
     float* s_delta = s_lse + kStep;
     float* s_bias = reinterpret_cast<float*>(reinterpret_cast<char*>(s_raw) + W * kStage);
@@ -529,7 +535,24 @@ __global__ __launch_bounds__(kWave* W)
             s_bias[i] = static_cast<float>(table[(axis * a.buckets + b) * a.heads + c * a.share + hs]) * kLog2e;
         }
     }
-    if (W > 1 && kBias) __syncthreads();
+    // Unit vectors of the keys' cells (the waves' are the same), and the tables for them.
+    const int axis_pairs = kBias ? key_axis_pairs<T>(a) : 0, pair_words = 2 * axis_pairs * table_words(a.reach);
+    Vec8<T>* s_units = reinterpret_cast<Vec8<T>*>(s_bias + (a.share * entries + 3) / 4 * 4);
+    uint32_t* s_pair = reinterpret_cast<uint32_t*>(s_units + axis_pairs * KT * kWave);
+    const int table_bytes = E == 2 ? entries * 4 : 1;
+    const float unscale = 1.0f / a.scale;
+    bool quick = false;
+    if constexpr (kBias && E == 2) {
+        quick = axis_pairs > 0 && unscalable(a.scale);
+        for (int hs = 0; hs < a.share; ++hs) {
+            const bool small = fill_pairs(s_pair + hs * pair_words, a, c * a.share + hs, axis_pairs, true, threadIdx.x,
+                                          kWave * W);
+            quick = quick && small;
+        }
+        quick = __syncthreads_and(quick);
+    } else if constexpr (kBias && W > 1) {
+        __syncthreads();
+    }
     Vec8<T> kf[KT][DS], vf[KT][DS];
     int kc[KT][3];
     {
@@ -563,7 +586,15 @@ __global__ __launch_bounds__(kWave* W)
             }
             k_least[x] = least_lane(lo);
             k_most[x] = largest_lane(hi);
+            if constexpr (E == 2) quick = quick && k_most[x] - k_least[x] < 4 * kWindow;
         }
+    }
+    if constexpr (kBias && E == 2) {
+        for (int m = 0; m < axis_pairs; ++m)
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt)
+                s_units[(m * KT + kt) * kWave + lane] =
+                    unit_slots<T>(m == 0 ? (g < 2 ? kc[kt][0] - k_least[0] : kc[kt][1] - k_least[1]) : kc[kt][2] - k_least[2], g);
     }
     f32x4 dk[KT][DT], dv[KT][DT];
 #pragma unroll
@@ -621,7 +652,7 @@ __global__ __launch_bounds__(kWave* W)
                 lse = real ? a.lse[h * a.q_total + mine] : HUGE_VALF;
                 delta = real ? gr.delta[h * a.q_total + mine] : 0.0f;
                 if constexpr (kBias) {
-                    head = hs * entries * 4;
+                    head = E == 2 ? hs : hs * entries * 4;
 #pragma unroll
                     for (int x = 0; x < 3; ++x)
                         if (x < a.axes) cells[x] = a.q_cells[mine * a.axes + x];
@@ -654,7 +685,7 @@ __global__ __launch_bounds__(kWave* W)
                 lse = real ? a.lse[h * a.q_total + mine] : HUGE_VALF;
                 delta = real ? gr.delta[h * a.q_total + mine] : 0.0f;
                 if constexpr (kBias) {
-                    head = (h - c * a.share) * entries * 4;
+                    head = (h - c * a.share) * (E == 2 ? 1 : entries * 4);
 #pragma unroll
                     for (int x = 0; x < 3; ++x)
                         if (x < a.axes) cells[x] = a.q_cells[mine * a.axes + x];
@@ -686,8 +717,32 @@ __global__ __launch_bounds__(kWave* W)
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
+                for (int kt = 0; kt < KT; ++kt) p[rt][kt] = ds[rt][kt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            if constexpr (kBias && E == 2) {
+                if (quick) {
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) {
+                        const uint32_t* pairs = s_pair + s_head[16 * rt + n] * pair_words;
+#pragma unroll
+                        for (int m = 0; m < 2; ++m) {
+                            if (m >= axis_pairs) continue;
+                            const int axis = 2 * m + (g >> 1);
+                            const int low = m == 0 ? (g < 2 ? k_least[0] : k_least[1]) : k_least[2];
+                            const Vec8<T> of =
+                                pair_slots(pairs, a, axis, g, low - s_cell[min(axis, a.axes - 1) * kStep + 16 * rt + n]);
+#pragma unroll
+                            for (int kt = 0; kt < KT; ++kt)
+                                p[rt][kt] = mma(of, s_units[(m * KT + kt) * kWave + lane], p[rt][kt]);
+                        }
+#pragma unroll
+                        for (int kt = 0; kt < KT; ++kt) p[rt][kt] *= unscale;
+                    }
+                }
+            }
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
                 for (int kt = 0; kt < KT; ++kt) {
-                    p[rt][kt] = ds[rt][kt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                     for (int s = 0; s < DS; ++s) {
                         p[rt][kt] = mma(qf[rt][s], kf[kt][s], p[rt][kt]);
@@ -696,7 +751,7 @@ __global__ __launch_bounds__(kWave* W)
                 }
             // Whether no distance of the step is clamped.
             bool close[3] = {};
-            if constexpr (kBias) {
+            if (kBias && !quick) {
 #pragma unroll
                 for (int x = 0; x < 3; ++x) {
                     if (x >= a.axes) continue;
@@ -713,9 +768,9 @@ __global__ __launch_bounds__(kWave* W)
                 for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) p[rt][kt][r] = __builtin_fmaf(p[rt][kt][r], to_log2, -l[r]);
-                if constexpr (kBias) {
+                if (kBias && !quick) {
                     const int4 hd = *reinterpret_cast<const int4*>(s_head + 16 * rt + 4 * g);
-                    const int heads[4] = {hd.x, hd.y, hd.z, hd.w};
+                    const int heads[4] = {hd.x * table_bytes, hd.y * table_bytes, hd.z * table_bytes, hd.w * table_bytes};
 #pragma unroll
                     for (int x = 0; x < 3; ++x) {
                         if (x >= a.axes) continue;
@@ -865,8 +920,12 @@ hipError_t launch_dkv_waves(const AttendArgs& a, const AttendGrads& g, hipStream
     constexpr int kKeys = 16 * key_tiles<T>(DP);
     const int tiles = (a.k_block + kKeys - 1) / kKeys;
     const int64_t items = static_cast<int64_t>(a.blocks) * tiles * a.kv_heads;
+    const size_t pairs = kBias ? key_axis_pairs<T>(a) : 0;
     const size_t stage = W * (2 * kStep * turned_stride<T>(DP) * sizeof(T) + 6 * kStep * sizeof(float)) +
-                         (kBias ? static_cast<size_t>(a.share) * a.axes * (2 * a.reach + 1) * sizeof(float) : 0);
+                         (kBias ? (static_cast<size_t>(a.share) * a.axes * (2 * a.reach + 1) + 3) / 4 * 4 * sizeof(float) +
+                                      pairs * key_tiles<T>(DP) * kWave * 8 * sizeof(T) +
+                                      a.share * 2 * pairs * table_words(a.reach) * sizeof(uint32_t)
+                                : 0);
     const size_t parts = W > 1 ? static_cast<size_t>(W) * key_tiles<T>(DP) * (DP / 16) * 8 * kWave * sizeof(float) : 0;
     const size_t lds = std::max(stage, parts);
     const auto kernel = attend_dkv_kernel<T, DP, W, kBias, kWhole>;
