@@ -84,9 +84,12 @@ __global__ __launch_bounds__(kWave* W) __attribute__((amdgpu_waves_per_eu(forwar
         }
     }
     uint32_t* s_pair = reinterpret_cast<uint32_t*>(s_bias + a.share * entries);
-    bool small = true;
-    if constexpr (kBias && E == 2) small = fill_pairs(s_pair, a, c, axis_pairs, false, threadIdx.x, kWave * W);
-    if constexpr (kBias) small = __syncthreads_and(small);
+    bool small = false;
+    if constexpr (kBias && E == 2) {
+        small = __syncthreads_and(fill_pairs(s_pair, a, c, axis_pairs, false, threadIdx.x, kWave * W));
+    } else if constexpr (kBias) {
+        __syncthreads();
+    }
 
     const float to_log2 = a.scale * kLog2e;
     Vec8<T> qf[RT][DS];
