@@ -43,10 +43,11 @@ __host__ __device__ __forceinline__ bool by_products(const AttendArgs& a) {
 // time.  With 242 registers two waves share a SIMD: the products take 0.25 ms of its
 // cycles, the vector instructions (the softmax, one exponential a score) 0.35 ms, and
 // two waves overlap these and the loads only in part.  Locality of the choice does not
-// count (the same blocks for all rows: no faster).  With a bias (16 clouds of 10,000
-// points, 8 blocks, 4 heads of 32 channels, two axes: 202 us) the table's lookups in
-// LDS and their adds, two a score, take over.  fp32's products run at an eighth of the
-// rate and need 64 channels a tile at most (see launch_rows).
+// count (the same blocks for all rows: no faster), nor do a fifth fewer vector
+// instructions (1.4 % faster).  With a bias, 16 clouds of 10,000 points, 8 blocks, 4
+// heads of 32 channels, two axes take 162 us; with a lookup in LDS and an add for every
+// score and axis instead of the product 202 us.  fp32, whose products run at an eighth
+// of the rate, keeps the lookups.
 template <typename T, int DP, int RT, int W, bool kBias, bool kExact>
 __global__ __launch_bounds__(kWave* W) __attribute__((amdgpu_waves_per_eu(forward_waves<T>(DP, RT, W, kBias || kExact)))) void attend_kernel(AttendArgs a, int tiles, int64_t items) {
     constexpr int DS = DP / 32, DT = DP / 16, KT = kChunk / 16, E = sizeof(T);

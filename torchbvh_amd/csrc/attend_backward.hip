@@ -17,13 +17,14 @@ constexpr int kStep = 32;  // rows of the other side per step
 
 // Waves of the query-side kernel with a bias, over all heads: each takes many tiles
 // of one head, so that few parts of the table's gradient are left to add up, and all
-// run at once, two a SIMD (a training step over 77,000 points: 2.21 ms, with 4096 waves
-// 2.42, with 8192 2.31; over 37,000 in fp32: 0.93, 1.03, 0.95).
+// run at once, two a SIMD (a training step over 77,000 points, at the time: 2.21 ms, with
+// 4096 waves 2.42, with 8192 2.31; over 37,000 in fp32: 0.93, 1.03, 0.95).
 constexpr int kTableWaves = 2048;
 
 // Key tiles up to this many waves are split between four waves each: blocks are chosen
 // unequally often, and a wave alone with a long run keeps the launch waiting (77,000
-// points, 8 heads, 16 blocks: 749 us, with one wave a tile 862).  Beyond, the
+// points, 8 heads, 16 blocks: 749 us, with one wave a tile 862, before the bias's
+// products).  Beyond, the
 // tiles themselves even that out.
 constexpr int64_t kSplitWaves = 1 << 16;
 
@@ -78,11 +79,12 @@ __device__ __forceinline__ Vec8<T> units(const int* cells, int g, int at) {
 // list of them: tiles part, part + parts, ... of one head.
 //
 // 77,000 points in 8 clouds, 16 blocks of 64, 8 heads of 32 channels, bf16, three axes:
-// 1030 us.  The vector instructions issue in half of the cycles (a lookup and an add a
-// score and axis, the exponential, the unit vectors, the joins of ds and its rest);
-// the table's gradient is 30 % of the time; two waves a SIMD (254 registers) leave a
-// fifth of it waiting for LDS and loads.  fp32 (37,000 points, 4 heads of 24 channels):
-// 405 us, half of its cycles in the products, of which the unit vectors' are a third.
+// 850 us (1030 with a lookup and an add for every score and axis instead of the bias's
+// products).  The vector instructions are active in 60 % of the cycles (the exponential,
+// the keys' unit vectors, the joins of ds and its rest), the products in 20 %; the
+// table's gradient is a third of the time; two waves a SIMD (256 registers).  fp32
+// (37,000 points, 4 heads of 24 channels): 410 us, half of its cycles in the products,
+// of which the unit vectors' are a third.
 template <typename T, int DP, int RT, bool kBias>
 __global__ __launch_bounds__(kWave)
     __attribute__((amdgpu_waves_per_eu(query_waves(sizeof(T), DP, RT)))) void attend_dq_kernel(AttendArgs a, AttendGrads gr,
@@ -495,9 +497,11 @@ __host__ __device__ __forceinline__ int key_axis_pairs(const AttendArgs& a) {
 // W waves take every W-th step, and their sums are added in order.
 //
 // Keys and sums stay in registers, 32 keys of each head: the rows are read again by
-// every key block that they chose, out of the L2 (77,000 points as above: 750 us, the
-// vector instructions and LDS's turned reads of q and grad each half of the cycles; 64
-// keys a wave spilled and were slower).  A row's weights p and its ds are rounded to T
+// every key block that they chose, out of the L2 (77,000 points as above: 708 us; the
+// vector instructions are active in 56 % of the cycles, LDS, mostly the turned reads of
+// q and grad, in a third, the products in 16 %; 64 keys a wave spilled and were
+// slower).  Three waves a SIMD at five spilled registers are faster than two without
+// (the step 1.88 against 2.08 ms).  A row's weights p and its ds are rounded to T
 // once for their products.
 template <typename T, int DP, int W, bool kBias, bool kWhole>
 __global__ __launch_bounds__(kWave* W)
